@@ -57,6 +57,19 @@ class WordStats(C.Structure):
                 ("list_entries", C.c_uint64), ("table_scans", C.c_uint64), ("bytes", C.c_uint64)]
 
 
+class Logits(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("dtype", C.c_uint32), ("n_rows", C.c_uint32), ("n_bias", C.c_uint32), ("logits", C.c_void_p),
+                ("row_stride", C.c_uint64), ("history", C.c_void_p), ("history_stride", C.c_uint64), ("lengths", C.c_void_p),
+                ("prompt_lengths", C.c_void_p), ("history_cap", C.c_uint32), ("n_mask_rows", C.c_uint32), ("repetition", C.c_void_p),
+                ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias_tokens", C.c_void_p), ("biases", C.c_void_p),
+                ("bias_stride", C.c_uint64), ("mask", C.c_void_p), ("mask_stride", C.c_uint64), ("mask_rows", C.c_void_p)]
+
+
+class Choice(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("reserved", C.c_uint32), ("uniform", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+                ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("tokens_out", C.c_void_p), ("logprobs_out", C.c_void_p)]
+
+
 PROGRESS_CB = C.CFUNCTYPE(None, C.POINTER(Progress), C.c_void_p)
 
 # name → (restype, argtypes); also the list of symbols the header declares
@@ -109,6 +122,16 @@ SIGNATURES = {
     "b200bpe_decoder_run": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64, u64p]),
     "b200bpe_decoder_read": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64]),
     "b200bpe_decoder_destroy": (None, [C.c_void_p]),
+    "b200bpe_sampler_create": (C.c_int32, [C.c_void_p, C.c_uint32, C.POINTER(C.c_void_p)]),
+    "b200bpe_sampler_adjust": (C.c_int32, [C.c_void_p, C.POINTER(Logits), C.c_void_p, C.c_uint64, C.c_void_p]),
+    "b200bpe_sampler_sample": (C.c_int32, [C.c_void_p, C.POINTER(Logits), C.POINTER(Choice), C.c_void_p]),
+    "b200bpe_sampler_destroy": (None, [C.c_void_p]),
+    "b200bpe_grammar_create": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32,
+                                           C.POINTER(C.c_void_p)]),
+    "b200bpe_grammar_mask": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "b200bpe_grammar_advance": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32,
+                                            C.c_void_p, C.c_void_p, C.c_void_p]),
+    "b200bpe_grammar_destroy": (None, [C.c_void_p]),
     "b200bpe_replay_create": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint32, C.POINTER(C.c_void_p)]),
     "b200bpe_replay_encode": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, u64p]),
     "b200bpe_replay_encode_device": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, u64p]),

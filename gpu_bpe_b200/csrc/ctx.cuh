@@ -129,6 +129,24 @@ struct CtxHold {
     ~CtxHold();
 };
 
+// For the length of a call: the context's device is the current one; the caller's is so again afterwards.
+struct OnDevice {
+    int before = -1;
+    cudaError_t error;
+    explicit OnDevice(int device) {
+        error = cudaGetDevice(&before);
+        if (error == cudaSuccess && before != device) error = cudaSetDevice(device);
+        else before = -1;
+    }
+    ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
+};
+
+// BAD_ARG, with the reason as the last error's text.
+inline b200bpe_status refused(const char* why) {
+    set_last_error(why);
+    return B200BPE_ERR_BAD_ARG;
+}
+
 b200bpe_status load_nccl(const char* path, NcclApi* api);
 
 // Ask the L2 to keep [base, base + bytes) resident for the kernels launched on the context's

@@ -157,6 +157,16 @@ class TrieTokenizer:
             out += bytes(self._vocab[t] if t < len(self._vocab) else UTF8_REPLACEMENT)
         return bytes(out)
 
+    def sampler(self):
+        """TokenSampler for logits over this vocabulary."""
+        from .token_sampler import TokenSampler
+        return TokenSampler(self._engine, len(self._vocab))
+
+    def grammar(self, transitions, accepting, endToken: int | None = None):
+        """TokenGrammar of a byte automaton over this vocabulary as it is now."""
+        from .token_grammar import TokenGrammar
+        return TokenGrammar(self._engine, self._vocab, transitions, accepting, endToken)
+
     def destroy(self):
         with self._decode_lock:
             self._drop_decoder()

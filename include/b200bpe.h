@@ -10,7 +10,8 @@
  * different handles are.  One context drives one GPU; multi-GPU jobs run one process (or thread)
  * per GPU and join their contexts with b200bpe_ctx_create_dist.
  *
- * All integers are little-endian unsigned; no floating point is computed on the path.
+ * All integers are little-endian unsigned; no floating point is computed on the paths of training and
+ * encoding.  The choice of the next token, further down, takes a model's logits.
  */
 #ifndef B200BPE_H
 #define B200BPE_H
@@ -270,6 +271,92 @@ b200bpe_status b200bpe_decoder_decode(b200bpe_decoder*, const uint32_t* tokens, 
 b200bpe_status b200bpe_decoder_run(b200bpe_decoder*, const uint32_t* tokens, uint64_t n, uint64_t* n_bytes_out);
 b200bpe_status b200bpe_decoder_read(b200bpe_decoder*, uint8_t* out, uint64_t cap);
 void b200bpe_decoder_destroy(b200bpe_decoder*);
+
+/* ── the next token: from a model's logits over the vocabulary to a token id (no counterpart in the reference, whose tokens end in
+ * decode) ──
+ * All pointers are device pointers on the context's GPU.  The calls only enqueue: `stream` is the caller's cudaStream_t (NULL is CUDA's default
+ * stream), nothing is allocated, copied or waited for, and a handle holds no memory that a call writes; so calls can be captured into graphs, and
+ * any number of threads, streams and graphs can use one handle at a time.  Inputs are only read, and have to stay as they are until the work is
+ * done; outputs must not overlap inputs, but for logits_out, which may be the logits themselves.  What a pointer's data says is taken as it
+ * is: nothing in it makes a call fail or read out of range. */
+enum { B200BPE_F32 = 0, B200BPE_F16 = 1, B200BPE_BF16 = 2 };
+#define B200BPE_NO_TOKEN 0xFFFFFFFFu   /* a row without a token that could be chosen */
+#define B200BPE_NO_STATE 0xFFFFFFFFu   /* a grammar's state behind a token that it does not allow */
+
+/* One row of logits for each request, and what changes them.  x = logits in 32 bits; each step is rounded to 32 bits:
+ *   for tokens of the row's history (the first lengths[r] entries of history's row; ids outside the vocabulary are skipped)
+ *     x = x > 0 ? x / repetition : x * repetition,
+ *   and, with c occurrences from prompt_lengths[r] on, c > 0:  x = x - frequency * c, then x = x - presence;
+ *   x = x + bias for the row's listed tokens (one that is listed twice gets both, in the order of the list; ids outside the vocabulary are
+ *   unused places);
+ *   x = -infinity where the row's mask has a 0.  Bit v & 31 of word v >> 5 is token v's. */
+typedef struct {
+    uint32_t struct_size;           /* sizeof(b200bpe_logits); zero-initialise */
+    uint32_t dtype;                 /* B200BPE_F32, _F16 or _BF16 */
+    uint32_t n_rows;
+    uint32_t n_bias;                /* places of a row's list, at most 1,024 */
+    const void* logits;             /* n_rows x at least the vocabulary's size; columns behind it are not looked at */
+    uint64_t row_stride;            /* elements from a row to the next (the same for all strides: elements of their arrays) */
+    const uint32_t* history;        /* NULL: no history */
+    uint64_t history_stride;
+    const uint32_t* lengths;        /* n_rows; more than history_cap counts as history_cap */
+    const uint32_t* prompt_lengths; /* n_rows, or NULL: 0 */
+    uint32_t history_cap;           /* entries that a row of history has room for */
+    uint32_t n_mask_rows;           /* rows of mask */
+    const float* repetition;        /* n_rows each, or NULL: 1, 0, 0 */
+    const float* presence;
+    const float* frequency;
+    const uint32_t* bias_tokens;    /* n_rows x n_bias */
+    const float* biases;
+    uint64_t bias_stride;           /* of both */
+    const uint32_t* mask;           /* NULL: all tokens are allowed */
+    uint64_t mask_stride;
+    const uint32_t* mask_rows;      /* which row of mask is row r's, or NULL: r.  n_mask_rows or more: no token is allowed */
+} b200bpe_logits;
+
+/* How a row's token is chosen from its x.  A NaN counts as -infinity; what is -infinity is never chosen.  With m = max x and
+ * w = exp((x - m) / temperature): of the top_k largest x, of those the shortest run from the largest on that has at least top_p of their weight,
+ * of those the tokens with w >= min_p (ties: the lowest id comes first) the first, in order of ids, at which the running sum of w is above
+ * uniform times the sum.  A temperature below 2^-16 (or NaN): the largest x.  Sums that decide are those of weights in 64 bits. */
+typedef struct {
+    uint32_t struct_size;           /* sizeof(b200bpe_choice); zero-initialise */
+    uint32_t reserved;
+    const float* uniform;           /* n_rows, each in [0, 1) (others count as the nearest, NaN as 0); NULL: every row takes its largest x */
+    const float* temperature;       /* n_rows, or NULL: 1 */
+    const uint32_t* top_k;          /* n_rows, or NULL: 0.  0: all */
+    const float* top_p;             /* n_rows, or NULL: 1.  1 or more, or NaN: all; 0 or less: one token */
+    const float* min_p;             /* n_rows, or NULL: 0.  0 or less, or NaN: all; more than 1 counts as 1 */
+    uint32_t* tokens_out;           /* n_rows; B200BPE_NO_TOKEN where no token is allowed */
+    float* logprobs_out;            /* n_rows, or NULL: log of the token's share of the weights of all tokens of the row, before top_k, top_p and
+                                       min_p (temperature 1 where the largest x is taken); -infinity without a token */
+} b200bpe_choice;
+
+typedef struct b200bpe_sampler b200bpe_sampler;
+/* vocab_size: 1 to 458,752 tokens (a row's x stays on chip, shared out over a cluster's memory). */
+b200bpe_status b200bpe_sampler_create(b200bpe_ctx*, uint32_t vocab_size, b200bpe_sampler** out);
+/* The x of every row, rounded once to the logits' type.  Columns behind the vocabulary are left as they are. */
+b200bpe_status b200bpe_sampler_adjust(b200bpe_sampler*, const b200bpe_logits*, void* logits_out, uint64_t out_stride, void* stream);
+/* Both steps in one kernel: x stays on chip. */
+b200bpe_status b200bpe_sampler_sample(b200bpe_sampler*, const b200bpe_logits*, const b200bpe_choice*, void* stream);
+void b200bpe_sampler_destroy(b200bpe_sampler*);
+
+/* A grammar over a vocabulary: a deterministic automaton that reads bytes.  Host arrays: the vocabulary as b200bpe_decoder_create takes it,
+ * transitions[s * 256 + byte] (n_states or more: there is none), accepting[s] (not 0: a text may end here), 1 to 65,535 states.  end_token
+ * stands for the end of a text, whatever its bytes are (n_entries or more: no token does). */
+typedef struct b200bpe_grammar b200bpe_grammar;
+b200bpe_status b200bpe_grammar_create(b200bpe_ctx*, const uint8_t* bytes, const uint64_t* offsets, uint32_t n_entries, const uint32_t* transitions,
+                                      const uint8_t* accepting, uint32_t n_states, uint32_t end_token, b200bpe_grammar** out);
+/* The tokens that the grammar allows in each of n_rows states, as rows of a mask: those with bytes, all of which have a transition, and the end
+ * token in an accepting state.  A state outside the grammar allows none.  Bits behind the vocabulary are 0; mask_stride is in words, at
+ * least one for each 32 entries; words behind those are left as they are. */
+b200bpe_status b200bpe_grammar_mask(b200bpe_grammar*, const uint32_t* states, uint32_t n_rows, uint32_t* mask_out, uint64_t mask_stride, void* stream);
+/* The step behind a choice: states_out[r] (may be states) is the state behind tokens[r]; B200BPE_NO_STATE if there is none; the end token
+ * leaves an accepting state as it is, and B200BPE_NO_TOKEN any.  With a history (NULL: none), tokens[r] also becomes entry lengths[r] of its row and
+ * lengths_out[r] (may be lengths) is one more; B200BPE_NO_TOKEN, and a row with history_cap entries, changes neither. */
+b200bpe_status b200bpe_grammar_advance(b200bpe_grammar*, const uint32_t* states, const uint32_t* tokens, uint32_t n_rows, uint32_t* states_out,
+                                       uint32_t* history, uint64_t history_stride, uint32_t history_cap, const uint32_t* lengths,
+                                       uint32_t* lengths_out, void* stream);
+void b200bpe_grammar_destroy(b200bpe_grammar*);
 
 /* ── merge-replay encoding: replaces TokenizerManager.encode (src/ui/tokenizer-manager.js:13-61) ──
  * The reference's other encoder: one token per byte, then every merge rule {a, b, new_id} applied in the order
