@@ -19,7 +19,7 @@ namespace cg = cooperative_groups;
 
 namespace b200bpe {
 
-constexpr int SM_THREADS = 512;
+constexpr int SM_THREADS = 256;
 constexpr int SM_WARPS = SM_THREADS / 32;
 constexpr uint32_t SM_MAX_CLUSTER = 8;           // portable size
 constexpr uint32_t SM_MAX_SLICE = 53248;         // 208 KB of 32-bit values
@@ -114,17 +114,85 @@ __device__ __forceinline__ uint32_t mask_bits(const MaskRow& mask, int token, ui
     return __funnelshift_r(lo, w + 1 < words ? __ldg(mask.words + w + 1) : 0u, (uint32_t)token & 31u);
 }
 
-// Fills the slice with x.  SCRUB: a NaN becomes -infinity, and -0 becomes 0.  Called by all threads of the cluster; ends with a barrier of the CTA.
+// A warp's part of the slice: places [lo, hi).
+struct Span {
+    uint32_t lo, hi;
+    __device__ Span(uint32_t padded, uint32_t warp) {
+        const uint32_t each = (padded + SM_WARPS * 256 - 1) / (SM_WARPS * 256) * 256;
+        lo = min(each * warp, padded);
+        hi = min(lo + each, padded);
+    }
+};
+
+// A thread's largest x, the place of the first vector that has it, and the sum of 2^(x c - n) over its x, n being a whole number next to the largest
+// x c: sums with different n are brought to one another by powers of two, without rounding.
+struct Stats {
+    static constexpr float FAR = 8589934592.0f;      // 2^33: where x c lies further out, neighbouring floats are 512 powers of two apart
+    float c, m = -INFINITY, n = -FAR;
+    uint32_t at = 0;
+    double sum = 0;
+    static __device__ __forceinline__ float two_to(float y) {
+        float w;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(y));
+        return w;
+    }
+    // 2^e for a whole number e of at most 0.
+    static __device__ __forceinline__ double power(float e) { return e < -1000.0f ? 0.0 : __hiloint2double((1023 + (int)e) << 20, 0); }
+    __device__ __forceinline__ float base(float largest) const { return fminf(fmaxf(rintf(largest * c), -FAR), FAR); }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&v)[N], uint32_t p) {
+        float top = v[0];
+#pragma unroll
+        for (int k = 1; k < N; k++) top = fmaxf(top, v[k]);
+        if (top > m) {
+            m = top;
+            at = p;
+            const float to = base(top);
+            if (to > n) {
+                sum *= power(n - to);
+                n = to;
+            }
+        }
+        float w[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) w[k] = two_to(fmaf(v[k], c, -n));
+#pragma unroll
+        for (int o = 1; o < N; o *= 2)
+#pragma unroll
+            for (int k = 0; k + o < N; k += 2 * o) w[k] += w[k + o];
+        sum += (double)w[0];
+    }
+};
+// The same of a slice that is there.
+template <class S>
+__device__ __forceinline__ void slice_stats(const Slice& s, S& stats) {
+    const Span span(s.padded, threadIdx.x >> 5);
+    for (uint32_t p = span.lo + (threadIdx.x & 31) * 4; p < span.hi; p += 128) {
+        const float4 x = *reinterpret_cast<const float4*>(s.buf + p);
+        const float v[4] = {x.x, x.y, x.z, x.w};
+        stats.add(v, p);
+    }
+}
+struct NoStats {
+    template <int N>
+    __device__ __forceinline__ void add(const float (&)[N], uint32_t) {}
+};
+
+// Fills the slice with x.  With statistics (taken on the way if there are no biases), a NaN becomes -infinity, and -0 becomes 0.  Called by all
+// threads of the cluster; ends with a barrier of the CTA.
 // The first loads of the row are on their way while the history is counted: a call with one row waits for little else.
-template <class T, bool SCRUB>
-__device__ void load_slice(const b200bpe_logits& in, uint32_t vocab, const Slice& s) {
-    constexpr uint32_t N = Packed<T>::N, AHEAD = 4, STEP = SM_THREADS * N;
+template <class T, class S>
+__device__ __forceinline__ void load_slice(const b200bpe_logits& in, uint32_t vocab, const Slice& s, S& stats) {
+    constexpr bool SCRUB = !std::is_same<S, NoStats>::value;
+    constexpr uint32_t N = Packed<T>::N, AHEAD = 8, STEP = 32 * N;
     const float lowest = -INFINITY;
     const T* row = static_cast<const T*>(in.logits) + (uint64_t)s.row * in.row_stride + s.lo;
+    const Span span(s.padded, threadIdx.x >> 5);
+    const uint32_t begin = span.lo + (threadIdx.x & 31) * N;
     uint4 q[AHEAD];
 #pragma unroll
     for (uint32_t j = 0; j < AHEAD; j++)
-        if (threadIdx.x * N + j * STEP < s.padded) q[j] = fetch(row, s, threadIdx.x * N + j * STEP);
+        if (begin + j * STEP < span.hi) q[j] = fetch(row, s, begin + j * STEP);
     const MaskRow mask = mask_row(in, s.row);
     Penalty pen{1.0f, 0.0f, 0.0f};
     uint32_t n_seen = 0;
@@ -152,13 +220,13 @@ __device__ void load_slice(const b200bpe_logits& in, uint32_t vocab, const Slice
         }
         cluster.sync();
     }
-    for (uint32_t p0 = threadIdx.x * N; p0 < s.padded; p0 += AHEAD * STEP) {
+    for (uint32_t p0 = begin; p0 < span.hi; p0 += AHEAD * STEP) {
 #pragma unroll
         for (uint32_t j = 0; j < AHEAD; j++) {
             const uint32_t p = p0 + j * STEP;
-            if (p >= s.padded) break;
+            if (p >= span.hi) break;
             const Packed<T> now{q[j]};
-            if (p + AHEAD * STEP < s.padded) q[j] = fetch(row, s, p + AHEAD * STEP);
+            if (p + AHEAD * STEP < span.hi) q[j] = fetch(row, s, p + AHEAD * STEP);
             const uint32_t allowed = mask_bits<N>(mask, (int)(s.lo + p) - (int)s.lead, vocab);
             float v[N];
 #pragma unroll
@@ -181,6 +249,7 @@ __device__ void load_slice(const b200bpe_logits& in, uint32_t vocab, const Slice
                 }
                 *reinterpret_cast<float4*>(s.buf + p + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
             }
+            if (SCRUB && !in.n_bias) stats.add(v, p);
         }
     }
     __syncthreads();
@@ -201,6 +270,7 @@ __device__ void load_slice(const b200bpe_logits& in, uint32_t vocab, const Slice
             s.x()[t - s.lo] = v;
         }
         __syncthreads();
+        if (SCRUB) slice_stats(s, stats);
     }
 }
 
@@ -222,11 +292,12 @@ __device__ Slice slice_of(const b200bpe_logits& in, uint32_t vocab, float* buf) 
 
 // ── adjusted logits ──
 template <class T>
-__global__ void __launch_bounds__(SM_THREADS)
+__global__ void __launch_bounds__(SM_THREADS, 3)
 k_adjust(const __grid_constant__ b200bpe_logits in, uint32_t vocab, T* out, uint64_t out_stride) {
     extern __shared__ __align__(16) float buf[];
     const Slice s = slice_of<T>(in, vocab, buf);
-    load_slice<T, false>(in, vocab, s);
+    NoStats none;
+    load_slice<T>(in, vocab, s, none);
     // Places that lie on 16 bytes in the logits do so in the output if its rows are aligned like the logits' (in place, and with equal strides).
     constexpr uint32_t N = Packed<T>::N;
     T* to = out + (uint64_t)s.row * out_stride + s.lo;
@@ -263,26 +334,25 @@ __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float
 
 constexpr uint32_t LOWEST_KEY = 0x007FFFFFu;     // of -infinity
 constexpr uint32_t SM_BINS = 2048;
-constexpr uint32_t SM_CANDIDATES = 1024;
+constexpr uint32_t SM_CANDIDATES = 1024, SM_EACH = SM_CANDIDATES / SM_THREADS;
+constexpr uint32_t SM_QUICK_K = 512;             // top_k up to which a row's candidates are looked for without bins
 
 // Which token is chosen depends on sums of weights: on the first running sum that is above a border.  Sums are made of weights in 32 bits,
-// w = 2^y with y = (x - m) * (log2 e / temperature), and added in 64 bits: y is off by at most three roundings, 3 * 2^-24 |y|, and the exponential
-// by 2^-22 of itself; four weights are added in 32 bits first, two more roundings.  So no sum is further off than
-//     E = sum w * (2^-22 + 2^-23 + 3 * 2^-24 * ln 2 * |y|),
-// and where a border lies within 2 E (E of the sum, E of the border, which is a share of another one) of a sum that decides, the row's sums are made
-// again of weights in 64 bits.  An exponential in 64 bits is some 18 operations at half the rate of those in 32, against 5 and a quarter of a special one.
+// w = 2^(x c - n) with c = log2 e / temperature, and added in 64 bits.  Against the exact weights, up to a factor that all have in common, the
+// exponent is off by the roundings of c and of the product's difference, together 2 * 2^-24 (m - x) c + 2^-24, the exponential by 2^-22 of itself, and up to
+// eight weights are added in 32 bits first, three roundings: a sum is off by at most
+//     E = sum w * 2^-24 * (8 + 2 ln 2 (m - x) c).
+// The mean of (m - x) c under the weights is their entropy less log2 Z, Z = sum w / max w, so at most log2(tokens / Z).  A border that is a share u of
+// the sum S has its part of the same errors: a running sum s is off from u S by (1 - u) times what s is off less u times what the rest is off, less than
+// E.  Where a running sum that decides lies within E of the border, the row's sums are made again of weights in 64 bits.
 struct Weights {
-    float m, c;         // the largest x, log2 e / temperature
+    float m, c, n;      // the largest x, log2 e / temperature, the exponent that all weights are relative to
     double by;          // 1 / temperature
-    __device__ __forceinline__ float power(float x) const { return fmaxf(fminf((x - m) * c, 0.0f), -150.0f); }   // (inf - inf is 0)
-    __device__ __forceinline__ float quick(float x) const { return two_to(power(x)); }
-    static __device__ __forceinline__ float two_to(float y) {
-        float w;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(y));
-        return w;
-    }
-    __device__ __forceinline__ double log_of(float x) const { return x == m ? 0.0 : ((double)x - (double)m) * by; }
-    __device__ __forceinline__ double exact(float x) const { return x == m ? 1.0 : exp(log_of(x)); }
+    __device__ __forceinline__ float quick(float x) const { return Stats::two_to(fmaf(x, c, -n)); }
+    // relative to the largest
+    __device__ __forceinline__ double log_of(float x) const { return ((double)x - (double)m) * by; }
+    __device__ __forceinline__ double exact(float x) const { return exp(log_of(x)); }
+    __device__ __forceinline__ double to_largest() const { return exp2((double)n - (double)m * (double)c); }        // quick's unit in exact's
 };
 
 // What of the row is kept: x with a larger key, and those with the key in front of token `end`.
@@ -294,18 +364,19 @@ struct Kept {
     }
 };
 
-struct Best { float x; uint32_t at; };
+struct Best { float m, n; uint32_t at, pad; double sum; float cut[4]; };       // a CTA's part of what the first exchange brings
 
 struct Shared {
-    Best best_warp[SM_WARPS], best_cta[SM_MAX_CLUSTER];
+    Best best[SM_MAX_CLUSTER];
     double part_warp[2][SM_WARPS], part_cta[2][2][SM_MAX_CLUSTER];      // (the second index: one exchange and the next)
     double scan_warp[SM_WARPS], warp_mass[SM_WARPS];
-    float cut_cta[2][SM_MAX_CLUSTER];
-    uint32_t border[2], candidates, flag, place, cut[2];
+    float m_warp[SM_WARPS], n_warp[SM_WARPS], cut[4];
+    uint32_t border[2], candidates, quick_candidates, flag, place, at, cut_at[2];
     Kept kept;
     union {
         uint32_t bins[SM_BINS];
         unsigned long long list[SM_CANDIDATES];      // candidates: key << 32 | ~token
+        uint32_t keys[SM_THREADS];
     };
 };
 
@@ -376,23 +447,17 @@ struct Team {
     }
 };
 
-// A warp's part of the slice: places [lo, hi), in steps of 128, four to a lane.
-struct Span {
-    uint32_t lo, hi;
-    __device__ Span(uint32_t padded, int warp) {
-        const uint32_t each = (padded + SM_WARPS * 128 - 1) / (SM_WARPS * 128) * 128;
-        lo = min(each * warp, padded);
-        hi = min(lo + each, padded);
-    }
-};
-
+// f(place, four x) for all of a warp's part, with all lanes (some of them behind the end, with -infinity).
 template <class F>
 __device__ __forceinline__ void each_four(const Slice& sl, int warp, F f) {
     const Span span(sl.padded, warp);
-    for (uint32_t p = span.lo + (threadIdx.x & 31) * 4; p < span.hi; p += 128) f(p, *reinterpret_cast<const float4*>(sl.buf + p));
+    for (uint32_t p0 = span.lo; p0 < span.hi; p0 += 128) {
+        const uint32_t p = p0 + (threadIdx.x & 31) * 4;
+        f(p, p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY));
+    }
 }
 
-// Sum of f over a row's kept places, with weights in 64 bits or in 32.
+// Sum of the weights of a row's kept places, as parts of the largest one: of weights in 64 bits or in 32.
 template <bool EXACT>
 __device__ __forceinline__ double kept_mass(const Slice& sl, int warp, const Weights& w, const Kept& kept) {
     double sum = 0;
@@ -405,7 +470,7 @@ __device__ __forceinline__ double kept_mass(const Slice& sl, int warp, const Wei
             else sum += (double)(((a ? w.quick(x.x) : 0.0f) + (b ? w.quick(x.y) : 0.0f)) + ((c ? w.quick(x.z) : 0.0f) + (d ? w.quick(x.w) : 0.0f)));
         }
     });
-    return sum;
+    return EXACT ? sum : sum * w.to_largest();
 }
 
 // The first place of the slice at which base plus the running sum of f(place, x) is above target; if there is none, the last with f above 0.  Every
@@ -487,17 +552,40 @@ __device__ void sort_down(unsigned long long* a, uint32_t n) {
         }
 }
 
-// Bins of x, from the largest downwards: SM_BINS of them over `range`; the last one takes the rest.
+// Bins of x, from the largest downwards: SM_BINS of them over `range`, each round its middle; the last one takes the rest.
 struct Bins {
     float m, scale;
     __device__ Bins(float largest, double range) : m(largest), scale((float)(SM_BINS / fmin(range, 3.4e38))) {}
-    __device__ __forceinline__ uint32_t of(float x) const { return min(__float2uint_rz((m - x) * scale), SM_BINS - 1); }   // (not a number is 0)
-    // x's weight in parts of 2^16 of its bin's largest, where a bin is 1/64 wide: e^-r by its first terms, rounded down.
-    __device__ __forceinline__ uint32_t weight_of(float x, uint32_t bin) const {
-        const float r = fmaxf((m - x) * scale - (float)bin, 0.0f) * (1.0f / 64);
-        return __float2uint_rz(65536.0f - 65536.0f * r + 32768.0f * r * r);
+    static __device__ __forceinline__ uint32_t whole(float x) { return __float_as_uint(x + 8388608.0f) & 0x7FFFFFu; }        // of 0 to 2^22, to the nearest
+    __device__ __forceinline__ float at(float x) const { return fminf((m - x) * scale, (float)(SM_BINS - 1)); }
+    __device__ __forceinline__ uint32_t of(float x) const { return whole(at(x)); }
+    // The weight of what lies at `at`, in parts of 2^16 of the middle of its bin, where a bin is 1/64 wide: e^-r by its first terms.
+    static __device__ __forceinline__ uint32_t weight(float at, uint32_t bin) {
+        const float r = at - (float)bin;
+        return whole(fmaf(fmaf(r, 8.0f, -1024.0f), r, 65536.0f));
     }
 };
+
+// Appends a lane's values whose bits are set in `in`, of tokens from v0 on, to the list of the cluster's first CTA, as far as there is room.
+__device__ __forceinline__ void gather(Team& t, uint32_t* counter, unsigned long long* list, const float (&v)[4], uint32_t in, uint32_t v0) {
+    if (!__any_sync(0xFFFFFFFFu, in != 0u)) return;
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t b = __ballot_sync(0xFFFFFFFFu, in >> k & 1u);
+        before += __popc(b & ((1u << t.lane) - 1u));
+        all += __popc(b);
+    }
+    uint32_t base = 0;
+    if (t.lane == 0) base = atomicAdd(counter, all);
+    base = __shfl_sync(0xFFFFFFFFu, base, 0) + before;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (in >> k & 1u) {
+            if (base < SM_CANDIDATES) list[base] = (unsigned long long)key_of(v[k]) << 32 | (uint32_t)~(v0 + k);
+            base++;
+        }
+}
 
 // The part of the row's order at which a running sum, from the largest x on, reaches `target`: of weights (MASS) or of tokens.
 // s.bins are filled in all CTAs (weights: in parts of 2^16 of the bin's largest), and a barrier of the cluster is behind that.
@@ -510,9 +598,10 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     const uint32_t mine = SM_BINS / t.C, per = max(mine / SM_THREADS, 1u), first = t.rank * mine + threadIdx.x * per;
     const bool busy = threadIdx.x * per < mine;
     double here[SM_BINS / SM_THREADS], sum = 0;
-    for (uint32_t k = 0; k < per; k++) {
+#pragma unroll
+    for (uint32_t k = 0; k < SM_BINS / SM_THREADS; k++) {
         here[k] = 0;
-        if (busy) {
+        if (busy && k < per) {
             unsigned long long n = 0;
             for (uint32_t c = 0; c < t.C; c++) n += t.peer(c)->bins[first + k];
             here[k] = MASS ? (double)n * exp(-(double)(first + k) / 64) / 65536.0 : (double)n;
@@ -526,8 +615,10 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     double a = threadIdx.x == 0 ? all : 0.0, none = 0;
     t.total(a, none);
     for (uint32_t c = 0; c < t.rank; c++) at += t.part(0, c);
-    const double slack = MASS ? 4.0 / 65536 : 0.0;          // of a bin's parts, and of the weights
-    for (uint32_t k = 0; k < per && busy; k++) {
+    const double slack = MASS ? 1.0 / 32768 : 0.0;          // 2^-17 a weight, 2 * 2^-24 * 2048 / 64 its place, and what the target is off
+#pragma unroll
+    for (uint32_t k = 0; k < SM_BINS / SM_THREADS; k++) {
+        if (k >= per || !busy) break;
         const double next = at + here[k];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
@@ -545,21 +636,18 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
         const float v[4] = {x.x, x.y, x.z, x.w};
         float part = 0;
+        uint32_t in = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const uint32_t b = bins.of(v[k]);
-            if (v[k] == -INFINITY || b > to) continue;
-            if (b < from) {
-                if (MASS) part += w.quick(v[k]);
-                else part += 1.0f;
-            } else {
-                const uint32_t n = atomicAdd(&lead->candidates, 1u);
-                // (the list lies where the first CTA's bins were)
-                if (n < SM_CANDIDATES) lead->list[n] = (unsigned long long)key_of(v[k]) << 32 | (uint32_t)~(p + k + shift);
-            }
+            if (b < from) part += MASS ? w.quick(v[k]) : 1.0f;
+            else if (b <= to && v[k] > -INFINITY) in |= 1u << k;
         }
         above += (double)part;
+        // (the list lies where the first CTA's bins were)
+        gather(t, &lead->candidates, lead->list, v, in, p + shift);
     });
+    if (MASS) above *= w.to_largest();
     t.total(above, count);
     const uint32_t n = t.peer(0)->candidates;
     if (n <= SM_CANDIDATES) {
@@ -573,17 +661,18 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                     __syncthreads();
                     sort_down(s.list, size);
                 }
-                // two neighbours to a thread; flag 1: a sum was near, 2: the bins were misjudged
-                double v[2];
-                for (int k = 0; k < 2; k++) {
-                    const uint32_t i = threadIdx.x * 2 + k;
+                // neighbours to a thread; flag 1: a sum was near, 2: the bins were misjudged
+                double v[SM_EACH], mine = 0;
+                for (uint32_t k = 0; k < SM_EACH; k++) {
+                    const uint32_t i = threadIdx.x * SM_EACH + k;
                     v[k] = i < n ? (MASS ? w.exact(value_of((uint32_t)(s.list[i] >> 32))) : 1.0) : 0.0;
+                    mine += v[k];
                 }
                 if (threadIdx.x == 0) { s.flag = 0u; s.place = n ? n - 1 : 0u; }
-                double ignored, sum = above + t.before(v[0] + v[1], &ignored);
-                for (int k = 0; k < 2; k++) {
+                double ignored, sum = above + t.before(mine, &ignored);
+                for (uint32_t k = 0; k < SM_EACH; k++) {
                     const double next = sum + v[k];
-                    const uint32_t i = threadIdx.x * 2 + k;
+                    const uint32_t i = threadIdx.x * SM_EACH + k;
                     if (i < n && sum < target && next >= target) s.place = i;
                     if (MASS && turn == 0 && i < n && (fabs(sum - target) <= margin || fabs(next - target) <= margin)) s.flag = 1u;
                     sum = next;
@@ -596,11 +685,11 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                     Shared* p = t.peer(threadIdx.x);
                     const unsigned long long e = s.list[s.place];
                     p->kept = n ? Kept{(uint32_t)(e >> 32), ~(uint32_t)e + 1u} : Kept{LOWEST_KEY, 0u};
-                    p->cut[0] = s.flag;
+                    p->cut_at[0] = s.flag;
                 }
             }
             t.sync();
-            if (s.cut[0] == 0u) return s.kept;
+            if (s.cut_at[0] == 0u) return s.kept;
             if (turn == 1) break;
             // weights in 64 bits: of all, for the target, and of what is above
             double total = 0;
@@ -657,14 +746,90 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     if (t.rank == owner) {
         bool near;
         const uint32_t p = find_place(t, sl, base, ties - 0.5, 0.0, &near, [&](uint32_t, float x) { return key_of(x) == low ? 1.0 : 0.0; });
-        if (threadIdx.x < t.C) t.peer(threadIdx.x)->cut[1] = p + shift + 1u;
+        if (threadIdx.x < t.C) t.peer(threadIdx.x)->cut_at[1] = p + shift + 1u;
     }
     t.sync();
-    return Kept{low, s.cut[1]};
+    return Kept{low, s.cut_at[1]};
+}
+
+struct Settings {
+    bool greedy;
+    double warm;            // temperature
+    uint32_t top_k;         // 0: all
+    float top_p, min_p, uniform;
+    __device__ Settings(const b200bpe_choice& how, uint32_t row, uint32_t vocab) {
+        const float t = how.temperature ? how.temperature[row] : 1.0f;
+        greedy = !how.uniform || !(t >= SM_GREEDY_BELOW);
+        warm = greedy ? 1.0 : fmin((double)t, 3.4e38);
+        top_k = greedy || !how.top_k ? 0u : how.top_k[row];
+        if (top_k >= vocab) top_k = 0u;
+        const float p = greedy || !how.top_p ? 1.0f : how.top_p[row], m = greedy || !how.min_p ? 0.0f : how.min_p[row];
+        top_p = p < 1.0f ? fmaxf(p, 0.0f) : 1.0f;
+        min_p = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
+        const float u = greedy ? 0.0f : how.uniform[row];
+        uniform = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
+    }
+    // The smallest x that min_p keeps.
+    __device__ uint32_t min_key(float m) const {
+        return min_p > 0.0f ? key_of(__double2float_ru((double)m + log((double)min_p) * warm) + 0.0f) : LOWEST_KEY;
+    }
+};
+
+// The choice among the candidates in the first CTA's list, which has all of the top_k largest: everything in 64 bits.  Called by that CTA's threads.
+__device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& set, uint32_t n, float* x) {
+    Shared& s = t.s;
+    uint32_t size = 2;
+    while (size < n) size *= 2;
+    for (uint32_t i = n + threadIdx.x; i < size; i += SM_THREADS) s.list[i] = 0ull;
+    __syncthreads();
+    sort_down(s.list, size);
+    n = min(n, set.top_k);
+    const uint32_t i0 = threadIdx.x * SM_EACH, min_key = set.min_key(w.m);
+    double v[SM_EACH], mine = 0, all;
+    for (uint32_t k = 0; k < SM_EACH; k++) {
+        v[k] = i0 + k < n ? w.exact(value_of((uint32_t)(s.list[i0 + k] >> 32))) : 0.0;
+        mine += v[k];
+    }
+    if (threadIdx.x == 0) s.place = 0u;
+    double sum = t.before(mine, &all);
+    const double enough = (double)set.top_p * all;
+    // what stays, with the token in front, so that the order becomes the tokens'
+    unsigned long long e[SM_EACH];
+    for (uint32_t k = 0; k < SM_EACH; k++) {
+        const unsigned long long c = i0 + k < n ? s.list[i0 + k] : 0ull;
+        const bool stays = i0 + k < n && (set.top_p >= 1.0f || sum < enough || i0 + k == 0u) && (uint32_t)(c >> 32) >= min_key;
+        e[k] = stays ? c << 32 | c >> 32 : 0ull;
+        sum += v[k];
+    }
+    __syncthreads();
+    for (uint32_t k = 0; k < SM_EACH; k++)
+        if (i0 + k < size) s.list[i0 + k] = e[k];
+    __syncthreads();
+    sort_down(s.list, size);
+    mine = 0;
+    uint32_t filled = 0;
+    for (uint32_t k = 0; k < SM_EACH; k++) {
+        const unsigned long long c = i0 + k < size ? s.list[i0 + k] : 0ull;
+        v[k] = c ? w.exact(value_of((uint32_t)c)) : 0.0;
+        if (v[k] > 0) filled = i0 + k;
+        mine += v[k];
+    }
+    if (filled) atomicMax(&s.place, filled);         // (without a sum above the target the last one)
+    sum = t.before(mine, &all);
+    const double target = (double)set.uniform * all;
+    __syncthreads();
+    for (uint32_t k = 0; k < SM_EACH; k++) {
+        if (v[k] > 0 && sum <= target && sum + v[k] > target) s.place = i0 + k;
+        sum += v[k];
+    }
+    __syncthreads();
+    const unsigned long long c = s.list[s.place];
+    *x = value_of((uint32_t)c);
+    return ~(uint32_t)(c >> 32);
 }
 
 template <class T>
-__global__ void __launch_bounds__(SM_THREADS, 2)
+__global__ void __launch_bounds__(SM_THREADS, 3)
 k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200bpe_choice how, uint32_t vocab) {
     extern __shared__ __align__(16) float buf[];
     __shared__ Shared s;
@@ -672,123 +837,206 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     cg::cluster_group cluster = cg::this_cluster();
     const Slice sl = slice_of<T>(in, vocab, buf);
     const int shift = (int)sl.lo - (int)sl.lead;
-    load_slice<T, true>(in, vocab, sl);
+    const Settings set(how, sl.row, vocab);
+    const bool by_k = set.top_k != 0u, by_p = set.top_p < 1.0f, quick_k = by_k && set.top_k <= SM_QUICK_K;
+    Stats stats;
+    stats.c = (float)(1.4426950408889634 / set.warm);
+    load_slice<T>(in, vocab, sl, stats);
     cluster.barrier_arrive();        // (nobody writes into a CTA that has not begun)
 
-    // the largest x, and the lowest token that has it
-    Best best{-INFINITY, 0xFFFFFFFFu};
-    each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
-        if (x.x > best.x) best = {x.x, p + shift};
-        if (x.y > best.x) best = {x.y, p + 1 + shift};
-        if (x.z > best.x) best = {x.z, p + 2 + shift};
-        if (x.w > best.x) best = {x.w, p + 3 + shift};
-    });
-    for (int turn = 0; turn < 2; turn++) {
+    // The first exchange: the largest x and the lowest token that has it, the sum of all weights, and for top_k a value that so many are not below.
+    float m, n;
+    double all;
+    for (bool again = false;; again = true) {
+        m = stats.m;
+        n = stats.n;
+        double sum = stats.sum;
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
-            const float x = __shfl_xor_sync(0xFFFFFFFFu, best.x, o);
-            const uint32_t at = __shfl_xor_sync(0xFFFFFFFFu, best.at, o);
-            if (x > best.x || (x == best.x && at < best.at)) best = {x, at};
+            const float to = fmaxf(n, __shfl_xor_sync(0xFFFFFFFFu, n, o));
+            sum *= Stats::power(n - to);
+            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            n = to;
+            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
         }
-        if (turn == 0) {
-            if (t.lane == 0) s.best_warp[t.warp] = best;
-            __syncthreads();
-            best = s.best_warp[t.lane % SM_WARPS];
+        __syncthreads();
+        if (t.lane == 0) { s.m_warp[t.warp] = m; s.n_warp[t.warp] = n; s.part_warp[0][t.warp] = sum; }
+        if (threadIdx.x == 0) { s.at = 0xFFFFFFFFu; s.quick_candidates = 0u; }
+        if (threadIdx.x < 4) s.cut[threadIdx.x] = -INFINITY;
+        if (quick_k) s.keys[threadIdx.x] = key_of(stats.m);
+        else if (by_k || by_p)
+            for (uint32_t i = threadIdx.x; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0u;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < SM_WARPS; i++) { m = fmaxf(m, s.m_warp[i]); n = fmaxf(n, s.n_warp[i]); }
+        if (stats.m == m && m > -INFINITY) {
+            uint32_t p = stats.at;
+            while (buf[p] != m) p++;
+            atomicMin(&s.at, p + shift);
         }
+        if (quick_k) {
+            uint32_t rank = 0;
+            const uint32_t mine = key_of(stats.m);
+            for (uint32_t i = 0; i < SM_THREADS; i += 4) {
+                const uint4 k = *reinterpret_cast<const uint4*>(s.keys + i);
+                rank += (k.x > mine || (k.x == mine && i < threadIdx.x)) + (k.y > mine || (k.y == mine && i + 1 < threadIdx.x)) +
+                        (k.z > mine || (k.z == mine && i + 2 < threadIdx.x)) + (k.w > mine || (k.w == mine && i + 3 < threadIdx.x));
+            }
+            // cut[l]: at least top_k / 2^l of this slice are not below it
+            for (int l = 0; l < 4; l++)
+                if (rank + 1u == (set.top_k + (1u << l) - 1u) >> l) s.cut[l] = stats.m;
+        }
+        __syncthreads();
+        if (!again) cluster.barrier_wait();
+        if (threadIdx.x < t.C) {
+            Best b{m, n, s.at, 0u, 0.0, {s.cut[0], s.cut[1], s.cut[2], s.cut[3]}};
+            for (int i = 0; i < SM_WARPS; i++) b.sum += s.part_warp[0][i] * Stats::power(s.n_warp[i] - n);
+            t.peer(threadIdx.x)->best[t.rank] = b;
+        }
+        t.sync();
+        for (uint32_t c = 0; c < t.C; c++) { m = fmaxf(m, s.best[c].m); n = fmaxf(n, s.best[c].n); }
+        if (again || m == -INFINITY || fabsf(m) * stats.c < Stats::FAR) break;
+        // So far out that only differences from m mean something.
+        for (uint32_t p = threadIdx.x; p < sl.padded; p += SM_THREADS) buf[p] = buf[p] == m ? 0.0f : m == INFINITY ? -INFINITY : buf[p] - m;
+        __syncthreads();
+        Stats near;
+        near.c = stats.c;
+        stats = near;
+        slice_stats(sl, stats);
+        t.sync();            // (what came is read)
     }
-    cluster.barrier_wait();
-    if (threadIdx.x < t.C) t.peer(threadIdx.x)->best_cta[t.rank] = best;
-    const float temperature = how.temperature ? how.temperature[sl.row] : 1.0f;
-    const bool greedy = !how.uniform || !(temperature >= SM_GREEDY_BELOW);
-    const uint32_t top_k = greedy || !how.top_k ? 0u : how.top_k[sl.row];
-    const float top_p = greedy || !how.top_p ? 1.0f : how.top_p[sl.row], min_p = greedy || !how.min_p ? 0.0f : how.min_p[sl.row];
-    const bool by_k = top_k != 0u && top_k < vocab, by_p = top_p < 1.0f;
-    if (by_k || by_p)
-        for (uint32_t i = threadIdx.x; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0u;
-    t.sync();
-    best = s.best_cta[0];
-    for (uint32_t c = 1; c < t.C; c++)
-        if (s.best_cta[c].x > best.x) best = s.best_cta[c];
-    if (best.x == -INFINITY) {          // (the whole cluster)
+    if (m == -INFINITY) {          // (the whole cluster)
         if (t.rank == 0 && threadIdx.x == 0) {
             how.tokens_out[sl.row] = B200BPE_NO_TOKEN;
             if (how.logprobs_out) how.logprobs_out[sl.row] = -INFINITY;
         }
         return;
     }
-    const double warm = greedy ? 1.0 : fmin((double)temperature, 3.4e38);
-    const Weights w{best.x, (float)(1.4426950408889634 / warm), 1.0 / warm};
-    // (what weighs less than e^-32 does not matter to top_p; it may to top_k, where a temperature is low)
-    const Bins k_bins(best.x, fmax(32.0 * warm, 24.0)), p_bins(best.x, 32.0 * warm);
-
-    // all weights; and the bins: of tokens for top_k, of weights for top_p
-    double all = 0, spread = 0;
-    each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
-        const float v[4] = {x.x, x.y, x.z, x.w};
-        float e[4], y[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            y[k] = w.power(v[k]);
-            e[k] = Weights::two_to(y[k]);
-            if (by_k) {
-                const uint32_t b = k_bins.of(v[k]);
-                if (b < SM_BINS - 1) atomicAdd(&s.bins[b], 1u);
-            } else if (by_p) {
-                const uint32_t b = p_bins.of(v[k]);
-                if (b < SM_BINS - 1) atomicAdd(&s.bins[b], p_bins.weight_of(v[k], b));
-            }
-        }
-        all += (double)((e[0] + e[1]) + (e[2] + e[3]));
-        spread -= (double)((e[0] * y[0] + e[1] * y[1]) + (e[2] * y[2] + e[3] * y[3]));
-    });
-    t.total(all, spread);
-    const double margin = 2.0 * (3.6e-7 * all + 1.25e-7 * spread);
-
-    Kept kept{LOWEST_KEY, 0u};
-    if (greedy) {
+    const Weights w{m, stats.c, n, 1.0 / set.warm};
+    const double unit = w.to_largest();
+    all = 0;
+    for (uint32_t c = 0; c < t.C; c++) all += s.best[c].sum * Stats::power(s.best[c].n - n);
+    all *= unit;
+    auto answer = [&](uint32_t token, float x) {
+        how.tokens_out[sl.row] = token;
+        if (how.logprobs_out) how.logprobs_out[sl.row] = (float)(w.log_of(x) - log(all));
+    };
+    if (set.greedy) {
         if (t.rank == 0 && threadIdx.x == 0) {
-            how.tokens_out[sl.row] = best.at;
-            if (how.logprobs_out) how.logprobs_out[sl.row] = (float)-log(all);
+            uint32_t token = 0xFFFFFFFFu;
+            for (uint32_t c = 0; c < t.C; c++)
+                if (s.best[c].m == m) token = min(token, s.best[c].at);
+            answer(token, m);
         }
         return;
     }
-    if (by_k) kept = border<false>(t, sl, w, k_bins, (double)top_k, -1.0, 0.0);
+    const double margin = all * (8.0 + 1.4 * (log2((double)vocab / all) + 1.0)) / 16777216.0;
+
+    // The kept tokens.
+    Kept kept{LOWEST_KEY, 0u};
+    if (quick_k) {
+        // At least top_k x are not below the largest value that 2^l of the CTAs have 1/2^l of top_k for.
+        float from = -INFINITY;
+        {
+            const uint32_t l = t.lane >> 3, c = t.lane & 7;
+            if (c < t.C && 1u << l <= t.C) {
+                const float mine = s.best[c].cut[l];
+                uint32_t so_many = 0;
+                for (uint32_t o = 0; o < t.C; o++) so_many += s.best[o].cut[l] >= mine;
+                if (so_many >= 1u << l) from = mine;
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) from = fmaxf(from, __shfl_xor_sync(0xFFFFFFFFu, from, o));
+        }
+        Shared* lead = t.peer(0);
+        each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
+            const float v[4] = {x.x, x.y, x.z, x.w};
+            uint32_t in = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) in |= (uint32_t)(v[k] >= from && v[k] > -INFINITY) << k;
+            gather(t, &lead->quick_candidates, lead->list, v, in, p + shift);
+        });
+        t.sync();
+        const uint32_t so_many = lead->quick_candidates;
+        cluster.barrier_arrive();
+        if (so_many <= SM_CANDIDATES) {
+            if (t.rank != 0) return;
+            float x;
+            const uint32_t token = choose_from_list(t, w, set, so_many, &x);
+            if (threadIdx.x == 0) answer(token, x);
+            cluster.barrier_wait();          // (the others have looked at the number)
+            return;
+        }
+        cluster.barrier_wait();
+        for (uint32_t i = threadIdx.x; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0u;
+        __syncthreads();
+    }
+    if (by_k) {
+        // (what weighs less than e^-32 does not matter to top_p; it may to top_k, where a temperature is low)
+        const Bins bins(m, fmax(32.0 * set.warm, 24.0));
+        each_four(sl, t.warp, [&](uint32_t, const float4& x) {
+            const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t b = bins.of(v[k]);
+                if (b < SM_BINS - 1) atomicAdd(&s.bins[b], 1u);
+            }
+        });
+        t.sync();
+        kept = border<false>(t, sl, w, bins, (double)set.top_k, -1.0, 0.0);
+    }
     if (by_p) {
         double whole = all, none = 0;
         if (by_k) {
-            // weights of the top_k alone, in 64 bits; their bins
             whole = kept_mass<true>(sl, t.warp, w, kept);
+            t.total(whole, none);
             for (uint32_t i = threadIdx.x; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0u;
             __syncthreads();
-            each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
+        }
+        Kept k{LOWEST_KEY, 0u};
+        if (set.top_p > 0.0f) {
+            const Bins bins(m, 32.0 * set.warm);
+            // All that lie lower than this weigh less than half of what top_p leaves out.
+            float lowest = (float)(SM_BINS - 1);
+            if (set.top_p < 0.999f) lowest = fminf(lowest, 64.0f * logf((float)((double)vocab / (0.5 * (1.0 - set.top_p) * whole))) + 1.0f);
+            each_four(sl, t.warp, [&](uint32_t, const float4& x) {
                 const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const uint32_t b = p_bins.of(v[k]);
-                    if (b < SM_BINS - 1) atomicAdd(&s.bins[b], p_bins.weight_of(v[k], b));
+                    const float at = bins.at(v[k]);
+                    if (at < lowest) {
+                        const uint32_t b = Bins::whole(at);
+                        atomicAdd(&s.bins[b], Bins::weight(at, b));
+                    }
                 }
             });
-            t.total(whole, none);
+            t.sync();
+            k = border<true>(t, sl, w, bins, (double)set.top_p * whole, by_k ? -1.0 : (double)set.top_p, margin);
+        } else {
+            uint32_t token = 0xFFFFFFFFu;
+            for (uint32_t c = 0; c < t.C; c++)
+                if (s.best[c].m == m) token = min(token, s.best[c].at);
+            k = {key_of(m), token + 1u};
         }
-        const double share = fmax((double)top_p, 0.0);
-        Kept k{key_of(best.x), best.at + 1u};
-        if (share > 0.0) k = border<true>(t, sl, w, p_bins, share * whole, by_k ? -1.0 : share, margin);
         if (k.key > kept.key || (k.key == kept.key && k.end < kept.end)) kept = k;
     }
-    if (min_p > 0.0f) {
-        const double least = (double)best.x + log((double)fminf(min_p, 1.0f)) * warm;
-        const uint32_t from = key_of(__double2float_ru(least) + 0.0f);
-        if (from > kept.key) kept = {from, 0xFFFFFFFFu};
-    }
+    const uint32_t min_key = set.min_key(m);
+    if (min_key > kept.key) kept = {min_key, 0xFFFFFFFFu};
 
-    // the draw
-    const float u = how.uniform[sl.row];
-    const double draw = u > 0.0f ? fmin((double)u, 1.0) : 0.0;
-    auto chosen = [&](auto exact, uint32_t* place) {         // whether this CTA has the token; -1: some sum was near
+    // The draw.
+    auto chosen = [&](auto exact, bool known, uint32_t* place) {         // whether this CTA has the token
         constexpr bool EXACT = decltype(exact)::value;
-        double mass = kept_mass<EXACT>(sl, t.warp, w, kept), none = 0;
-        t.total(mass, none);
-        const double target = draw * mass;
-        double base = 0;
+        if (known) {
+            if (threadIdx.x < t.C) s.part_cta[0][t.par][threadIdx.x] = s.best[threadIdx.x].sum * Stats::power(s.best[threadIdx.x].n - n) * unit;
+            if (threadIdx.x < SM_WARPS) s.warp_mass[threadIdx.x] = s.part_warp[0][threadIdx.x] * Stats::power(s.n_warp[threadIdx.x] - n) * unit;
+            __syncthreads();
+        } else {
+            double mass = kept_mass<EXACT>(sl, t.warp, w, kept), none = 0;
+            t.total(mass, none);
+        }
+        double mass = 0, base = 0;
+        for (uint32_t c = 0; c < t.C; c++) mass += t.part(0, c);
+        const double target = (double)set.uniform * mass;
         uint32_t owner = 0xFFFFFFFFu, filled = 0;
         for (uint32_t c = 0; c < t.C && owner == 0xFFFFFFFFu; c++) {
             if (t.part(0, c) > 0) filled = c;
@@ -803,20 +1051,17 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         if (t.rank == owner) {
             bool near;
             *place = find_place(t, sl, base, target, EXACT ? 0.0 : margin, &near, [&](uint32_t p, float x) {
-                return kept.has(x, p + shift) ? (EXACT ? w.exact(x) : (double)w.quick(x)) : 0.0;
+                return kept.has(x, p + shift) ? (EXACT ? w.exact(x) : (double)w.quick(x) * unit) : 0.0;
             });
-            if (!EXACT && threadIdx.x < t.C) t.peer(threadIdx.x)->cut[0] = near;
+            if (!EXACT && threadIdx.x < t.C) t.peer(threadIdx.x)->cut_at[0] = near;
         }
         if (!EXACT) t.sync();
         return t.rank == owner;
     };
     uint32_t place = 0;
-    bool mine = chosen(std::false_type{}, &place);
-    if (s.cut[0]) mine = chosen(std::true_type{}, &place);
-    if (mine && threadIdx.x == 0) {
-        how.tokens_out[sl.row] = place + shift;
-        if (how.logprobs_out) how.logprobs_out[sl.row] = (float)(w.log_of(buf[place]) - log(all));
-    }
+    bool mine = chosen(std::false_type{}, !by_k && !by_p && set.min_p == 0.0f, &place);
+    if (s.cut_at[0]) mine = chosen(std::true_type{}, false, &place);
+    if (mine && threadIdx.x == 0) answer(place + shift, buf[place]);
 }
 
 struct Sampler {
