@@ -21,9 +21,10 @@ namespace b200bpe {
 
 constexpr int SM_THREADS = 256;
 constexpr int SM_WARPS = SM_THREADS / 32;
-constexpr uint32_t SM_MAX_CLUSTER = 8;           // portable size
-constexpr uint32_t SM_MAX_SLICE = 53248;         // 208 KB of 32-bit values
+constexpr uint32_t SM_MAX_CLUSTER = 16;
+constexpr uint32_t SM_MAX_SLICE = 32768;         // 128 KB of 32-bit values
 constexpr uint32_t SM_MAX_VOCAB = SM_MAX_SLICE * SM_MAX_CLUSTER;
+constexpr uint32_t SM_ADJUST_SLICE = 8192;       // tokens that a CTA adjusts for a caller
 constexpr uint32_t SM_MAX_BIAS = 1024;
 constexpr float SM_GREEDY_BELOW = 1.0f / 65536;
 
@@ -47,12 +48,12 @@ __device__ __forceinline__ void rounded(float x, float* to) { *to = x; }
 __device__ __forceinline__ void rounded(float x, __half* to) { *to = __float2half_rn(x); }
 __device__ __forceinline__ void rounded(float x, __nv_bfloat16* to) { *to = __float2bfloat16_rn(x); }
 
-// One row's slice in a CTA: tokens [lo, lo + len) of row `row`; token lo + i lies at x[i].  x starts `lead` elements into the CTA's buffer, so that what is
+// One row's slice in a CTA: tokens [lo, lo + len) of row `row`; token lo + i lies `lead` + i elements into the CTA's buffer, so that what is
 // 16-byte aligned in the logits is so in the buffer, too; places in front of and behind the slice, up to `padded`, hold -infinity.
 struct Slice {
     uint32_t row, lo, len, lead, padded;
+    uint32_t inner;         // how many places, from the slice's first on, have all of their 16 bytes in it
     float* buf;
-    __device__ float* x() const { return buf + lead; }
 };
 
 // Tokens of a CTA's slice (the last ones may have fewer, or none): a multiple of 128, so that all slices of a row are aligned alike.
@@ -91,7 +92,7 @@ __device__ __forceinline__ MaskRow mask_row(const b200bpe_logits& in, uint32_t r
 template <class T>
 __device__ __forceinline__ uint4 fetch(const T* row, const Slice& s, uint32_t p) {
     constexpr uint32_t N = Packed<T>::N;
-    if (p >= s.lead && p + N <= s.lead + s.len) return __ldcs(reinterpret_cast<const uint4*>(row + (p - s.lead)));
+    if (p - s.lead < s.inner) return __ldcs(reinterpret_cast<const uint4*>(row + (p - s.lead)));
     T v[N];
 #pragma unroll
     for (uint32_t k = 0; k < N; k++) {
@@ -101,17 +102,6 @@ __device__ __forceinline__ uint4 fetch(const T* row, const Slice& s, uint32_t p)
     uint4 q;
     memcpy(&q, v, 16);
     return q;
-}
-
-// Bits of the N tokens from `token` on (a negative one: of those before the row) in the lowest bits.
-template <int N>
-__device__ __forceinline__ uint32_t mask_bits(const MaskRow& mask, int token, uint32_t vocab) {
-    if (mask.none) return 0u;
-    if (!mask.words) return 0xFFFFFFFFu;
-    const int w = token >> 5, words = (int)((vocab + 31u) / 32u);
-    const uint32_t lo = w >= 0 && w < words ? __ldg(mask.words + w) : 0u;
-    if (((uint32_t)token & 31u) + N <= 32u) return lo >> (token & 31);
-    return __funnelshift_r(lo, w + 1 < words ? __ldg(mask.words + w + 1) : 0u, (uint32_t)token & 31u);
 }
 
 // A warp's part of the slice: places [lo, hi).
@@ -124,6 +114,204 @@ struct Span {
     }
 };
 
+// Which places of a slice are not plain logits: bit p & 31 of word p >> 5 is place p's.
+template <uint32_t MOST>
+struct Special {
+    uint32_t seen[MOST / 32 + 1];        // in the history: the place itself holds its marks until x is there
+    uint32_t deny[MOST / 32 + 1];        // masked
+};
+
+// Makes `special` and the marks of the history.  Returns whether there are any special places.  Called by all threads of the CTA; ends with a barrier.
+// Each CTA reads the whole history of its row, and counts what is its own: a history is short beside a row, and L2 has it.
+template <uint32_t MOST>
+__device__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const Slice& s, const MaskRow& mask, Penalty& pen, Special<MOST>& special) {
+    uint32_t n_seen = 0, prompt = 0;
+    if (in.history) {
+        if (in.repetition) pen.repetition = in.repetition[s.row];
+        if (in.presence) pen.presence = in.presence[s.row];
+        if (in.frequency) pen.frequency = in.frequency[s.row];
+        if (pen.repetition != 1.0f || pen.presence != 0.0f || pen.frequency != 0.0f) {
+            n_seen = min(in.lengths[s.row], in.history_cap);
+            prompt = in.prompt_lengths ? in.prompt_lengths[s.row] : 0u;
+        }
+    }
+    if (n_seen == 0 && !mask.words && !mask.none) return false;
+    const uint32_t words = (s.padded + 31u) / 32u, mask_words = (vocab + 31u) / 32u;
+    for (uint32_t i = threadIdx.x; i < words; i += SM_THREADS) {
+        special.seen[i] = 0u;
+        uint32_t allowed = mask.none ? 0u : 0xFFFFFFFFu;
+        if (mask.words) {
+            const int v = (int)(s.lo + i * 32u) - (int)s.lead, w = v >> 5;
+            const uint32_t lo = w >= 0 && w < (int)mask_words ? mask.words[w] : 0u, hi = w + 1 < (int)mask_words ? mask.words[w + 1] : 0u;
+            allowed = __funnelshift_r(lo, hi, (uint32_t)v & 31u);
+        }
+        special.deny[i] = ~allowed;
+    }
+    __syncthreads();
+    if (n_seen) {
+        uint32_t* marks = reinterpret_cast<uint32_t*>(s.buf);
+        const uint32_t* h = in.history + (uint64_t)s.row * in.history_stride;
+        // first the places are emptied, then counted
+        for (int turn = 0; turn < 2; turn++) {
+            for (uint32_t i0 = threadIdx.x; i0 < n_seen; i0 += SM_THREADS * 4) {
+                uint32_t t[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) t[k] = i0 + k * SM_THREADS < n_seen ? h[i0 + k * SM_THREADS] - s.lo : 0xFFFFFFFFu;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (t[k] >= s.len) continue;
+                    const uint32_t p = t[k] + s.lead;
+                    if (turn == 0) {
+                        marks[p] = 0u;
+                        atomicOr(&special.seen[p >> 5], 1u << (p & 31u));
+                    } else if (i0 + k * SM_THREADS < prompt) {
+                        atomicOr(&marks[p], Penalty::SEEN);
+                    } else {
+                        atomicAdd(&marks[p], 1u);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+    return true;
+}
+
+// Calls to(place, N adjusted logits but for the biases) for the slice.  The first loads are the caller's (`ahead`, of first_loads): they are on their
+// way while special places are found, and a call with one row waits for little else.
+constexpr uint32_t SM_AHEAD = 4;
+template <class T>
+__device__ __forceinline__ void first_loads(const T* row, const Slice& s, uint4 (&ahead)[SM_AHEAD]) {
+    constexpr uint32_t N = Packed<T>::N;
+    const Span span(s.padded, threadIdx.x >> 5);
+#pragma unroll
+    for (uint32_t j = 0; j < SM_AHEAD; j++) {
+        const uint32_t p = span.lo + (threadIdx.x & 31) * N + j * 32 * N;
+        if (p < span.hi) ahead[j] = fetch(row, s, p);
+    }
+}
+template <class T, uint32_t MOST, class F>
+__device__ __forceinline__ void each_adjusted(const T* row, const Slice& s, uint4 (&ahead)[SM_AHEAD], bool any_special, const Special<MOST>& special,
+                                              const Penalty& pen, F to) {
+    constexpr uint32_t N = Packed<T>::N, STEP = 32 * N;
+    const Span span(s.padded, threadIdx.x >> 5);
+    for (uint32_t p0 = span.lo + (threadIdx.x & 31) * N; p0 < span.hi; p0 += SM_AHEAD * STEP) {
+#pragma unroll
+        for (uint32_t j = 0; j < SM_AHEAD; j++) {
+            const uint32_t p = p0 + j * STEP;
+            if (p >= span.hi) break;
+            const Packed<T> now{ahead[j]};
+            if (p + SM_AHEAD * STEP < span.hi) ahead[j] = fetch(row, s, p + SM_AHEAD * STEP);
+            float v[N];
+#pragma unroll
+            for (uint32_t k = 0; k < N; k++) v[k] = now.get(k);
+            if (any_special) {
+                constexpr uint32_t ALL = (1u << N) - 1u;
+                const uint32_t deny = special.deny[p >> 5] >> (p & 31u) & ALL, seen = special.seen[p >> 5] >> (p & 31u) & ALL;
+                if (deny | seen) {
+#pragma unroll
+                    for (uint32_t k = 0; k < N; k++) {
+                        if (seen >> k & 1u) v[k] = pen.on(v[k], reinterpret_cast<const uint32_t*>(s.buf)[p + k]);
+                        if (deny >> k & 1u) v[k] = -INFINITY;
+                    }
+                }
+            }
+            to(p, v);
+        }
+    }
+}
+template <int N>
+__device__ __forceinline__ void store(float* at, const float (&v)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(at + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+}
+
+// Adds the row's biases to the slice's x.  Called by all threads of the CTA, with a barrier in front; one has to follow.
+__device__ __forceinline__ void add_biases(const b200bpe_logits& in, const Slice& s, const MaskRow& mask) {
+    // Place i takes all biases of its token, unless an earlier place has that token.
+    const uint32_t* list = in.bias_tokens + (uint64_t)s.row * in.bias_stride;
+    const float* by = in.biases + (uint64_t)s.row * in.bias_stride;
+    for (uint32_t i = threadIdx.x; i < in.n_bias; i += SM_THREADS) {
+        const uint32_t t = list[i];
+        if (t < s.lo || t - s.lo >= s.len || !mask.allows(t)) continue;
+        bool first = true;
+        for (uint32_t j = 0; j < i; j++) first &= list[j] != t;
+        if (!first) continue;
+        float v = __fadd_rn(s.buf[s.lead + t - s.lo], by[i]);
+        for (uint32_t j = i + 1; j < in.n_bias; j++)
+            if (list[j] == t) v = __fadd_rn(v, by[j]);
+        s.buf[s.lead + t - s.lo] = v;
+    }
+}
+
+// Slice `part` of row `row`, of `whole` tokens but for the last ones.
+template <class T>
+__device__ __forceinline__ Slice slice_of(const b200bpe_logits& in, uint32_t vocab, uint32_t row, uint32_t part, uint32_t whole, float* buf) {
+    Slice s;
+    s.row = row;
+    s.lo = min(part * whole, vocab);
+    s.len = min(whole, vocab - s.lo);
+    const uint64_t at = reinterpret_cast<uint64_t>(static_cast<const T*>(in.logits) + (uint64_t)row * in.row_stride);
+    s.lead = (uint32_t)(at & 15u) / (uint32_t)sizeof(T);
+    s.padded = (s.lead + s.len + 7u) & ~7u;
+    s.inner = s.len >= Packed<T>::N ? s.len - Packed<T>::N + 1u : 0u;
+    s.buf = buf;
+    return s;
+}
+
+// ── adjusted logits ──
+template <class T>
+__device__ __forceinline__ void write_out(T* to, const Slice& s, bool alike, uint32_t p, const float (&x)[Packed<T>::N]) {
+    constexpr uint32_t N = Packed<T>::N;
+    T v[N];
+#pragma unroll
+    for (uint32_t k = 0; k < N; k++) rounded(x[k], v + k);
+    if (alike && p - s.lead < s.inner) {
+        uint4 q;
+        memcpy(&q, v, 16);
+        __stcs(reinterpret_cast<uint4*>(to + (p - s.lead)), q);
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < N; k++)
+            if (p + k >= s.lead && p + k < s.lead + s.len) to[p + k - s.lead] = v[k];
+    }
+}
+
+// A CTA for each slice of a row.  Bound by memory: a row is read and written once; only with biases does x pass through shared memory.
+template <class T>
+__global__ void __launch_bounds__(SM_THREADS, 4)
+k_adjust(const __grid_constant__ b200bpe_logits in, uint32_t vocab, T* out, uint64_t out_stride) {
+    extern __shared__ __align__(16) float buf[];
+    __shared__ Special<SM_ADJUST_SLICE + 8> special;
+    const uint32_t parts = (vocab + SM_ADJUST_SLICE - 1u) / SM_ADJUST_SLICE;
+    const Slice s = slice_of<T>(in, vocab, blockIdx.x / parts, blockIdx.x % parts, SM_ADJUST_SLICE, buf);
+    const T* row = static_cast<const T*>(in.logits) + (uint64_t)s.row * in.row_stride + s.lo;
+    uint4 ahead[SM_AHEAD];
+    first_loads(row, s, ahead);
+    const MaskRow mask = mask_row(in, s.row);
+    Penalty pen{1.0f, 0.0f, 0.0f};
+    const bool any_special = find_special(in, vocab, s, mask, pen, special);
+    T* to = out + (uint64_t)s.row * out_stride + s.lo;
+    // Places that lie on 16 bytes in the logits do so in the output if its rows are aligned like the logits' (in place, and with equal strides).
+    const bool alike = (reinterpret_cast<uint64_t>(to) & 15u) == s.lead * sizeof(T);
+    constexpr uint32_t N = Packed<T>::N;
+    if (!in.n_bias) {
+        each_adjusted(row, s, ahead, any_special, special, pen, [&](uint32_t p, float (&v)[N]) { write_out<T>(to, s, alike, p, v); });
+        return;
+    }
+    each_adjusted(row, s, ahead, any_special, special, pen, [&](uint32_t p, float (&v)[N]) { store(buf + p, v); });
+    __syncthreads();
+    add_biases(in, s, mask);
+    __syncthreads();
+    for (uint32_t p = threadIdx.x * N; p < s.padded; p += SM_THREADS * N) {
+        float v[N];
+#pragma unroll
+        for (uint32_t k = 0; k < N; k++) v[k] = buf[p + k];
+        write_out<T>(to, s, alike, p, v);
+    }
+}
+
+// ── the choice ──
 // A thread's largest x, the place of the first vector that has it, and the sum of 2^(x c - n) over its x, n being a whole number next to the largest
 // x c: sums with different n are brought to one another by powers of two, without rounding.
 struct Stats {
@@ -139,8 +327,9 @@ struct Stats {
     // 2^e for a whole number e of at most 0.
     static __device__ __forceinline__ double power(float e) { return e < -1000.0f ? 0.0 : __hiloint2double((1023 + (int)e) << 20, 0); }
     __device__ __forceinline__ float base(float largest) const { return fminf(fmaxf(rintf(largest * c), -FAR), FAR); }
+    // N x of place p on; a NaN among them becomes -infinity, in the buffer too.
     template <int N>
-    __device__ __forceinline__ void add(const float (&v)[N], uint32_t p) {
+    __device__ __forceinline__ void add(float (&v)[N], uint32_t p, float* buf) {
         float top = v[0];
 #pragma unroll
         for (int k = 1; k < N; k++) top = fmaxf(top, v[k]);
@@ -153,6 +342,17 @@ struct Stats {
                 n = to;
             }
         }
+        float w = weights(v);
+        if (w != w) {
+#pragma unroll
+            for (int k = 0; k < N; k++) v[k] = fmaxf(v[k], -INFINITY);       // (of a NaN and a number the number)
+            store(buf + p, v);
+            w = weights(v);
+        }
+        sum += (double)w;
+    }
+    template <int N>
+    __device__ __forceinline__ float weights(const float (&v)[N]) const {
         float w[N];
 #pragma unroll
         for (int k = 0; k < N; k++) w[k] = two_to(fmaf(v[k], c, -n));
@@ -160,174 +360,22 @@ struct Stats {
         for (int o = 1; o < N; o *= 2)
 #pragma unroll
             for (int k = 0; k + o < N; k += 2 * o) w[k] += w[k + o];
-        sum += (double)w[0];
+        return w[0];
     }
 };
 // The same of a slice that is there.
-template <class S>
-__device__ __forceinline__ void slice_stats(const Slice& s, S& stats) {
+__device__ __forceinline__ void slice_stats(const Slice& s, Stats& stats) {
     const Span span(s.padded, threadIdx.x >> 5);
     for (uint32_t p = span.lo + (threadIdx.x & 31) * 4; p < span.hi; p += 128) {
         const float4 x = *reinterpret_cast<const float4*>(s.buf + p);
-        const float v[4] = {x.x, x.y, x.z, x.w};
-        stats.add(v, p);
-    }
-}
-struct NoStats {
-    template <int N>
-    __device__ __forceinline__ void add(const float (&)[N], uint32_t) {}
-};
-
-// Fills the slice with x.  With statistics (taken on the way if there are no biases), a NaN becomes -infinity, and -0 becomes 0.  Called by all
-// threads of the cluster; ends with a barrier of the CTA.
-// The first loads of the row are on their way while the history is counted: a call with one row waits for little else.
-template <class T, class S>
-__device__ __forceinline__ void load_slice(const b200bpe_logits& in, uint32_t vocab, const Slice& s, S& stats) {
-    constexpr bool SCRUB = !std::is_same<S, NoStats>::value;
-    constexpr uint32_t N = Packed<T>::N, AHEAD = 8, STEP = 32 * N;
-    const float lowest = -INFINITY;
-    const T* row = static_cast<const T*>(in.logits) + (uint64_t)s.row * in.row_stride + s.lo;
-    const Span span(s.padded, threadIdx.x >> 5);
-    const uint32_t begin = span.lo + (threadIdx.x & 31) * N;
-    uint4 q[AHEAD];
-#pragma unroll
-    for (uint32_t j = 0; j < AHEAD; j++)
-        if (begin + j * STEP < span.hi) q[j] = fetch(row, s, begin + j * STEP);
-    const MaskRow mask = mask_row(in, s.row);
-    Penalty pen{1.0f, 0.0f, 0.0f};
-    uint32_t n_seen = 0;
-    if (in.history) {
-        if (in.repetition) pen.repetition = in.repetition[s.row];
-        if (in.presence) pen.presence = in.presence[s.row];
-        if (in.frequency) pen.frequency = in.frequency[s.row];
-        if (pen.repetition != 1.0f || pen.presence != 0.0f || pen.frequency != 0.0f) n_seen = min(in.lengths[s.row], in.history_cap);
-    }
-    // Every CTA of the cluster sees the same row, so all of them take the same branches round the cluster's barriers.
-    if (n_seen) {
-        cg::cluster_group cluster = cg::this_cluster();
-        uint32_t* marks = reinterpret_cast<uint32_t*>(s.buf);
-        for (uint32_t i = threadIdx.x * 4; i < s.padded; i += SM_THREADS * 4) *reinterpret_cast<uint4*>(marks + i) = make_uint4(0u, 0u, 0u, 0u);
-        cluster.sync();
-        const uint32_t* h = in.history + (uint64_t)s.row * in.history_stride;
-        const uint32_t prompt = in.prompt_lengths ? in.prompt_lengths[s.row] : 0u;
-        const uint32_t whole = slice_tokens(vocab, cluster.num_blocks());
-        for (uint32_t i = cluster.block_rank() * SM_THREADS + threadIdx.x; i < n_seen; i += cluster.num_blocks() * SM_THREADS) {
-            const uint32_t t = h[i];
-            if (t >= vocab) continue;
-            uint32_t* at = cluster.map_shared_rank(marks, t / whole) + s.lead + t % whole;
-            if (i < prompt) atomicOr(at, Penalty::SEEN);
-            else atomicAdd(at, 1u);
-        }
-        cluster.sync();
-    }
-    for (uint32_t p0 = begin; p0 < span.hi; p0 += AHEAD * STEP) {
-#pragma unroll
-        for (uint32_t j = 0; j < AHEAD; j++) {
-            const uint32_t p = p0 + j * STEP;
-            if (p >= span.hi) break;
-            const Packed<T> now{q[j]};
-            if (p + AHEAD * STEP < span.hi) q[j] = fetch(row, s, p + AHEAD * STEP);
-            const uint32_t allowed = mask_bits<N>(mask, (int)(s.lo + p) - (int)s.lead, vocab);
-            float v[N];
-#pragma unroll
-            for (uint32_t k = 0; k < N; k += 4) {
-                uint4 mark = make_uint4(0u, 0u, 0u, 0u);
-                if (n_seen) mark = *reinterpret_cast<const uint4*>(s.buf + p + k);
-                if (mark.x | mark.y | mark.z | mark.w) {
-                    v[k] = pen.on(now.get(k), mark.x);
-                    v[k + 1] = pen.on(now.get(k + 1), mark.y);
-                    v[k + 2] = pen.on(now.get(k + 2), mark.z);
-                    v[k + 3] = pen.on(now.get(k + 3), mark.w);
-                } else {
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; i++) v[k + i] = now.get(k + i);
-                }
-#pragma unroll
-                for (uint32_t i = 0; i < 4; i++) {
-                    if (!(allowed >> (k + i) & 1u)) v[k + i] = lowest;
-                    if (SCRUB) v[k + i] = fmaxf(v[k + i] + 0.0f, lowest);        // (of a NaN and a number the number)
-                }
-                *reinterpret_cast<float4*>(s.buf + p + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-            }
-            if (SCRUB && !in.n_bias) stats.add(v, p);
-        }
-    }
-    __syncthreads();
-    if (in.n_bias) {
-        // Place i takes all biases of its token, unless an earlier place has that token.
-        const uint32_t* list = in.bias_tokens + (uint64_t)s.row * in.bias_stride;
-        const float* by = in.biases + (uint64_t)s.row * in.bias_stride;
-        for (uint32_t i = threadIdx.x; i < in.n_bias; i += SM_THREADS) {
-            const uint32_t t = list[i];
-            if (t < s.lo || t - s.lo >= s.len || !mask.allows(t)) continue;
-            bool first = true;
-            for (uint32_t j = 0; j < i; j++) first &= list[j] != t;
-            if (!first) continue;
-            float v = __fadd_rn(s.x()[t - s.lo], by[i]);
-            for (uint32_t j = i + 1; j < in.n_bias; j++)
-                if (list[j] == t) v = __fadd_rn(v, by[j]);
-            if (SCRUB) v = fmaxf(v + 0.0f, lowest);
-            s.x()[t - s.lo] = v;
-        }
-        __syncthreads();
-        if (SCRUB) slice_stats(s, stats);
+        float v[4] = {x.x, x.y, x.z, x.w};
+        stats.add(v, p, s.buf);
     }
 }
 
-template <class T>
-__device__ Slice slice_of(const b200bpe_logits& in, uint32_t vocab, float* buf) {
-    cg::cluster_group cluster = cg::this_cluster();
-    const uint32_t C = cluster.num_blocks();
-    const uint32_t whole = slice_tokens(vocab, C);
-    Slice s;
-    s.row = blockIdx.x / C;
-    s.lo = min(cluster.block_rank() * whole, vocab);
-    s.len = min(whole, vocab - s.lo);
-    const uint64_t at = reinterpret_cast<uint64_t>(static_cast<const T*>(in.logits) + (uint64_t)s.row * in.row_stride);
-    s.lead = (uint32_t)(at & 15u) / (uint32_t)sizeof(T);
-    s.padded = (s.lead + s.len + 7u) & ~7u;
-    s.buf = buf;
-    return s;
-}
-
-// ── adjusted logits ──
-template <class T>
-__global__ void __launch_bounds__(SM_THREADS, 3)
-k_adjust(const __grid_constant__ b200bpe_logits in, uint32_t vocab, T* out, uint64_t out_stride) {
-    extern __shared__ __align__(16) float buf[];
-    const Slice s = slice_of<T>(in, vocab, buf);
-    NoStats none;
-    load_slice<T>(in, vocab, s, none);
-    // Places that lie on 16 bytes in the logits do so in the output if its rows are aligned like the logits' (in place, and with equal strides).
-    constexpr uint32_t N = Packed<T>::N;
-    T* to = out + (uint64_t)s.row * out_stride + s.lo;
-    const bool alike = (reinterpret_cast<uint64_t>(to) & 15u) == s.lead * sizeof(T);
-    for (uint32_t p = threadIdx.x * N; p < s.padded; p += SM_THREADS * N) {
-        T v[N];
-#pragma unroll
-        for (uint32_t k = 0; k < N; k += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(s.buf + p + k);
-            rounded(x.x, v + k);
-            rounded(x.y, v + k + 1);
-            rounded(x.z, v + k + 2);
-            rounded(x.w, v + k + 3);
-        }
-        if (alike && p >= s.lead && p + N <= s.lead + s.len) {
-            uint4 q;
-            memcpy(&q, v, 16);
-            __stcs(reinterpret_cast<uint4*>(to + (p - s.lead)), q);
-        } else {
-#pragma unroll
-            for (uint32_t k = 0; k < N; k++)
-                if (p + k >= s.lead && p + k < s.lead + s.len) to[p + k - s.lead] = v[k];
-        }
-    }
-}
-
-// ── the choice ──
 // The order of x as unsigned integers, and back.
 __device__ __forceinline__ uint32_t key_of(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.0f);        // (-0 is 0)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key); }
@@ -359,8 +407,8 @@ struct Weights {
 struct Kept {
     uint32_t key, end;
     __device__ __forceinline__ bool has(float x, uint32_t v) const {
-        const uint32_t k = key_of(x);
-        return k > key || (k == key && v < end);
+        const float at = value_of(key);
+        return x > at || (x == at && v < end);
     }
 };
 
@@ -377,6 +425,7 @@ struct Shared {
         uint32_t bins[SM_BINS];
         unsigned long long list[SM_CANDIDATES];      // candidates: key << 32 | ~token
         uint32_t keys[SM_THREADS];
+        Special<SM_MAX_SLICE + 8> special;           // until the slice is there
     };
 };
 
@@ -716,7 +765,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     auto from_key = [&](uint32_t key) {
         double mass = 0, none = 0;
         if (MASS) {
-            mass = kept_mass<true>(sl, t.warp, w, Kept{key - 1u, 0u});
+            mass = kept_mass<true>(sl, t.warp, w, Kept{key, 0xFFFFFFFFu});
         } else {
             each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
                 mass += (double)((key_of(x.x) >= key) + (key_of(x.y) >= key) + (key_of(x.z) >= key) + (key_of(x.w) >= key));
@@ -771,7 +820,7 @@ struct Settings {
     }
     // The smallest x that min_p keeps.
     __device__ uint32_t min_key(float m) const {
-        return min_p > 0.0f ? key_of(__double2float_ru((double)m + log((double)min_p) * warm) + 0.0f) : LOWEST_KEY;
+        return min_p > 0.0f ? key_of(__double2float_ru((double)m + log((double)min_p) * warm)) : LOWEST_KEY;
     }
 };
 
@@ -833,16 +882,33 @@ __global__ void __launch_bounds__(SM_THREADS, 3)
 k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200bpe_choice how, uint32_t vocab) {
     extern __shared__ __align__(16) float buf[];
     __shared__ Shared s;
-    Team t(s);
     cg::cluster_group cluster = cg::this_cluster();
-    const Slice sl = slice_of<T>(in, vocab, buf);
+    cluster.barrier_arrive();        // (nobody writes into a CTA that has not begun)
+    Team t(s);
+    const Slice sl = slice_of<T>(in, vocab, blockIdx.x / t.C, t.rank, slice_tokens(vocab, t.C), buf);
     const int shift = (int)sl.lo - (int)sl.lead;
+    const T* row = static_cast<const T*>(in.logits) + (uint64_t)sl.row * in.row_stride + sl.lo;
+    uint4 ahead[SM_AHEAD];
+    first_loads(row, sl, ahead);
     const Settings set(how, sl.row, vocab);
     const bool by_k = set.top_k != 0u, by_p = set.top_p < 1.0f, quick_k = by_k && set.top_k <= SM_QUICK_K;
     Stats stats;
     stats.c = (float)(1.4426950408889634 / set.warm);
-    load_slice<T>(in, vocab, sl, stats);
-    cluster.barrier_arrive();        // (nobody writes into a CTA that has not begun)
+    {
+        const MaskRow mask = mask_row(in, sl.row);
+        Penalty pen{1.0f, 0.0f, 0.0f};
+        const bool any_special = find_special(in, vocab, sl, mask, pen, s.special);
+        each_adjusted(row, sl, ahead, any_special, s.special, pen, [&](uint32_t p, float (&v)[Packed<T>::N]) {
+            store(buf + p, v);
+            if (!in.n_bias) stats.add(v, p, buf);
+        });
+        if (in.n_bias) {
+            __syncthreads();
+            add_biases(in, sl, mask);
+            __syncthreads();
+            slice_stats(sl, stats);
+        }
+    }
 
     // The first exchange: the largest x and the lowest token that has it, the sum of all weights, and for top_k a value that so many are not below.
     float m, n;
@@ -938,12 +1004,14 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         // At least top_k x are not below the largest value that 2^l of the CTAs have 1/2^l of top_k for.
         float from = -INFINITY;
         {
-            const uint32_t l = t.lane >> 3, c = t.lane & 7;
-            if (c < t.C && 1u << l <= t.C) {
-                const float mine = s.best[c].cut[l];
-                uint32_t so_many = 0;
-                for (uint32_t o = 0; o < t.C; o++) so_many += s.best[o].cut[l] >= mine;
-                if (so_many >= 1u << l) from = mine;
+            for (uint32_t i = t.lane; i < 4 * SM_MAX_CLUSTER; i += 32) {
+                const uint32_t l = i / SM_MAX_CLUSTER, c = i % SM_MAX_CLUSTER;
+                if (c < t.C && 1u << l <= t.C) {
+                    const float mine = s.best[c].cut[l];
+                    uint32_t so_many = 0;
+                    for (uint32_t o = 0; o < t.C; o++) so_many += s.best[o].cut[l] >= mine;
+                    if (so_many >= 1u << l) from = fmaxf(from, mine);
+                }
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) from = fmaxf(from, __shfl_xor_sync(0xFFFFFFFFu, from, o));
@@ -1096,17 +1164,18 @@ static b200bpe_status check_logits(const b200bpe_logits* in) {
 
 static uint32_t cluster_for(uint32_t vocab) {
     uint32_t c = 1;
-    while (c < SM_MAX_CLUSTER && vocab > c * 2048u) c *= 2;
+    while (c < 8 && vocab > c * 2048u) c *= 2;
+    while (c < SM_MAX_CLUSTER && vocab > c * 16384u) c *= 2;
     return c;
 }
 
-template <class K, class... A>
-static b200bpe_status launch(K kernel, uint32_t rows, uint32_t vocab, cudaStream_t stream, A... args) {
-    const uint32_t c = cluster_for(vocab), whole = slice_tokens(vocab, c);
+template <class T>
+static b200bpe_status launch_sample(const b200bpe_logits& in, const b200bpe_choice& how, uint32_t vocab, cudaStream_t stream) {
+    const uint32_t c = cluster_for(vocab);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(rows * c);
+    cfg.gridDim = dim3(in.n_rows * c);
     cfg.blockDim = dim3(SM_THREADS);
-    cfg.dynamicSmemBytes = (whole + 16) * 4;
+    cfg.dynamicSmemBytes = (slice_tokens(vocab, c) + 16) * 4;
     cfg.stream = stream;
     cudaLaunchAttribute a{};
     a.id = cudaLaunchAttributeClusterDimension;
@@ -1114,17 +1183,28 @@ static b200bpe_status launch(K kernel, uint32_t rows, uint32_t vocab, cudaStream
     a.val.clusterDim.y = a.val.clusterDim.z = 1;
     cfg.attrs = &a;
     cfg.numAttrs = 1;
-    B2_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    B2_CUDA(cudaLaunchKernelEx(&cfg, k_sample<T>, in, how, vocab));
+    return B200BPE_OK;
+}
+
+template <class T>
+static b200bpe_status launch_adjust(const b200bpe_logits& in, uint32_t vocab, void* out, uint64_t out_stride, cudaStream_t stream) {
+    const uint64_t parts = (vocab + SM_ADJUST_SLICE - 1) / SM_ADJUST_SLICE;
+    if (parts * in.n_rows > 0x7FFFFFFFu) return refused("b200bpe_sampler_adjust: too many rows");
+    const size_t bytes = in.history || in.n_bias ? (std::min(vocab, SM_ADJUST_SLICE) + 16) * 4 : 0;
+    k_adjust<T><<<(uint32_t)(parts * in.n_rows), SM_THREADS, bytes, stream>>>(in, vocab, static_cast<T*>(out), out_stride);
+    B2_CUDA(cudaGetLastError());
     return B200BPE_OK;
 }
 
 // Loads the kernels, so that no call has to, and lets them have a CTA's whole shared memory.
 static cudaError_t ready() {
-    const void* kernels[] = {(const void*)k_adjust<float>, (const void*)k_adjust<__half>, (const void*)k_adjust<__nv_bfloat16>,
-                             (const void*)k_sample<float>, (const void*)k_sample<__half>, (const void*)k_sample<__nv_bfloat16>};
-    for (const void* k : kernels) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (SM_MAX_SLICE + 16) * 4);
-        if (e != cudaSuccess) return e;
+    cudaFuncAttributes fa;
+    for (const void* k : {(const void*)k_adjust<float>, (const void*)k_adjust<__half>, (const void*)k_adjust<__nv_bfloat16>})
+        if (const cudaError_t e = cudaFuncGetAttributes(&fa, k)) return e;
+    for (const void* k : {(const void*)k_sample<float>, (const void*)k_sample<__half>, (const void*)k_sample<__nv_bfloat16>}) {
+        if (const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (SM_MAX_SLICE + 16) * 4)) return e;
+        if (const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
     }
     return cudaSuccess;
 }
@@ -1138,7 +1218,7 @@ using namespace b200bpe;
 extern "C" {
 
 b200bpe_status b200bpe_sampler_create(b200bpe_ctx* c, uint32_t vocab_size, b200bpe_sampler** out) {
-    if (vocab_size == 0 || vocab_size > SM_MAX_VOCAB) return refused("b200bpe_sampler_create: 1 to 425,984 tokens");
+    if (vocab_size == 0 || vocab_size > SM_MAX_VOCAB) return refused("b200bpe_sampler_create: 1 to 524,288 tokens");
     if (!c || !out) return refused("b200bpe_sampler_create: null pointer");
     const OnDevice on(c->c.device);
     B2_CUDA(on.error);
@@ -1165,9 +1245,9 @@ b200bpe_status b200bpe_sampler_adjust(b200bpe_sampler* h, const b200bpe_logits* 
     B2_CUDA(on.error);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (in->dtype) {
-        case B200BPE_F32: return launch(k_adjust<float>, in->n_rows, vocab, st, *in, vocab, static_cast<float*>(logits_out), out_stride);
-        case B200BPE_F16: return launch(k_adjust<__half>, in->n_rows, vocab, st, *in, vocab, static_cast<__half*>(logits_out), out_stride);
-        default: return launch(k_adjust<__nv_bfloat16>, in->n_rows, vocab, st, *in, vocab, static_cast<__nv_bfloat16*>(logits_out), out_stride);
+        case B200BPE_F32: return launch_adjust<float>(*in, vocab, logits_out, out_stride, st);
+        case B200BPE_F16: return launch_adjust<__half>(*in, vocab, logits_out, out_stride, st);
+        default: return launch_adjust<__nv_bfloat16>(*in, vocab, logits_out, out_stride, st);
     }
 }
 
@@ -1183,9 +1263,9 @@ b200bpe_status b200bpe_sampler_sample(b200bpe_sampler* h, const b200bpe_logits* 
     B2_CUDA(on.error);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (in->dtype) {
-        case B200BPE_F32: return launch(k_sample<float>, in->n_rows, vocab, st, *in, *how, vocab);
-        case B200BPE_F16: return launch(k_sample<__half>, in->n_rows, vocab, st, *in, *how, vocab);
-        default: return launch(k_sample<__nv_bfloat16>, in->n_rows, vocab, st, *in, *how, vocab);
+        case B200BPE_F32: return launch_sample<float>(*in, *how, vocab, st);
+        case B200BPE_F16: return launch_sample<__half>(*in, *how, vocab, st);
+        default: return launch_sample<__nv_bfloat16>(*in, *how, vocab, st);
     }
 }
 
