@@ -22,7 +22,7 @@ namespace b200bpe {
 constexpr int SM_THREADS = 256;
 constexpr int SM_WARPS = SM_THREADS / 32;
 constexpr uint32_t SM_MAX_CLUSTER = 16;
-constexpr uint32_t SM_MAX_SLICE = 32768;         // 128 KB of 32-bit values
+constexpr uint32_t SM_MAX_SLICE = 20480;         // 80 KB of 32-bit values
 constexpr uint32_t SM_MAX_VOCAB = SM_MAX_SLICE * SM_MAX_CLUSTER;
 constexpr uint32_t SM_ADJUST_SLICE = 8192;       // tokens that a CTA adjusts for a caller
 constexpr uint32_t SM_MAX_BIAS = 1024;
@@ -117,14 +117,17 @@ struct Span {
 // Which places of a slice are not plain logits: bit p & 31 of word p >> 5 is place p's.
 template <uint32_t MOST>
 struct Special {
-    uint32_t seen[MOST / 32 + 1];        // in the history: the place itself holds its marks until x is there
     uint32_t deny[MOST / 32 + 1];        // masked
+    uint32_t seen[MOST / 32 + 1];        // in the history: the buffer has its x
+    uint32_t todo[MOST / 32 + 1];        // not yet, it has its marks
 };
 
-// Makes `special` and the marks of the history.  Returns whether there are any special places.  Called by all threads of the CTA; ends with a barrier.
+// Makes `special`, and x of the places in the history: there, penalties cost a scattered load a token, not a test and a division for every lane of
+// the row.  Returns whether there are any special places.  Called by all threads of the CTA; ends with a barrier.
 // Each CTA reads the whole history of its row, and counts what is its own: a history is short beside a row, and L2 has it.
-template <uint32_t MOST>
-__device__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const Slice& s, const MaskRow& mask, Penalty& pen, Special<MOST>& special) {
+template <uint32_t MOST, class T>
+__device__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const T* row, const Slice& s, const MaskRow& mask, Special<MOST>& special) {
+    Penalty pen{1.0f, 0.0f, 0.0f};
     uint32_t n_seen = 0, prompt = 0;
     if (in.history) {
         if (in.repetition) pen.repetition = in.repetition[s.row];
@@ -138,7 +141,6 @@ __device__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const Sli
     if (n_seen == 0 && !mask.words && !mask.none) return false;
     const uint32_t words = (s.padded + 31u) / 32u, mask_words = (vocab + 31u) / 32u;
     for (uint32_t i = threadIdx.x; i < words; i += SM_THREADS) {
-        special.seen[i] = 0u;
         uint32_t allowed = mask.none ? 0u : 0xFFFFFFFFu;
         if (mask.words) {
             const int v = (int)(s.lo + i * 32u) - (int)s.lead, w = v >> 5;
@@ -146,29 +148,42 @@ __device__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const Sli
             allowed = __funnelshift_r(lo, hi, (uint32_t)v & 31u);
         }
         special.deny[i] = ~allowed;
+        special.seen[i] = special.todo[i] = 0u;
     }
+    uint32_t* marks = reinterpret_cast<uint32_t*>(s.buf);
+    if (n_seen)
+        for (uint32_t i = threadIdx.x * 4; i < s.padded; i += SM_THREADS * 4) *reinterpret_cast<uint4*>(marks + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     if (n_seen) {
-        uint32_t* marks = reinterpret_cast<uint32_t*>(s.buf);
         const uint32_t* h = in.history + (uint64_t)s.row * in.history_stride;
-        // first the places are emptied, then counted
+        // counted; then the first to come back to a place makes its x
         for (int turn = 0; turn < 2; turn++) {
             for (uint32_t i0 = threadIdx.x; i0 < n_seen; i0 += SM_THREADS * 4) {
                 uint32_t t[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) t[k] = i0 + k * SM_THREADS < n_seen ? h[i0 + k * SM_THREADS] - s.lo : 0xFFFFFFFFu;
+                if (turn == 0) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    if (t[k] >= s.len) continue;
-                    const uint32_t p = t[k] + s.lead;
-                    if (turn == 0) {
-                        marks[p] = 0u;
-                        atomicOr(&special.seen[p >> 5], 1u << (p & 31u));
-                    } else if (i0 + k * SM_THREADS < prompt) {
-                        atomicOr(&marks[p], Penalty::SEEN);
-                    } else {
-                        atomicAdd(&marks[p], 1u);
+                    for (int k = 0; k < 4; k++) {
+                        if (t[k] >= s.len) continue;
+                        const uint32_t p = t[k] + s.lead;
+                        const uint32_t had = i0 + k * SM_THREADS < prompt ? atomicOr(&marks[p], Penalty::SEEN) : atomicAdd(&marks[p], 1u);
+                        if (had == 0u) {
+                            atomicOr(&special.seen[p >> 5], 1u << (p & 31u));
+                            atomicOr(&special.todo[p >> 5], 1u << (p & 31u));
+                        }
                     }
+                } else {
+                    T x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (t[k] < s.len && !(atomicAnd(&special.todo[(t[k] + s.lead) >> 5], ~(1u << ((t[k] + s.lead) & 31u))) >> ((t[k] + s.lead) & 31u) & 1u))
+                            t[k] = 0xFFFFFFFFu;
+                        if (t[k] < s.len) x[k] = row[t[k]];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (t[k] < s.len) s.buf[t[k] + s.lead] = pen.on(as_float(x[k]), marks[t[k] + s.lead]);
                 }
             }
             __syncthreads();
@@ -192,7 +207,7 @@ __device__ __forceinline__ void first_loads(const T* row, const Slice& s, uint4 
 }
 template <class T, uint32_t MOST, class F>
 __device__ __forceinline__ void each_adjusted(const T* row, const Slice& s, uint4 (&ahead)[SM_AHEAD], bool any_special, const Special<MOST>& special,
-                                              const Penalty& pen, F to) {
+                                              F to) {
     constexpr uint32_t N = Packed<T>::N, STEP = 32 * N;
     const Span span(s.padded, threadIdx.x >> 5);
     for (uint32_t p0 = span.lo + (threadIdx.x & 31) * N; p0 < span.hi; p0 += SM_AHEAD * STEP) {
@@ -208,12 +223,19 @@ __device__ __forceinline__ void each_adjusted(const T* row, const Slice& s, uint
             if (any_special) {
                 constexpr uint32_t ALL = (1u << N) - 1u;
                 const uint32_t deny = special.deny[p >> 5] >> (p & 31u) & ALL, seen = special.seen[p >> 5] >> (p & 31u) & ALL;
-                if (deny | seen) {
+                if (seen) {
 #pragma unroll
-                    for (uint32_t k = 0; k < N; k++) {
-                        if (seen >> k & 1u) v[k] = pen.on(v[k], reinterpret_cast<const uint32_t*>(s.buf)[p + k]);
-                        if (deny >> k & 1u) v[k] = -INFINITY;
+                    for (uint32_t k = 0; k < N; k += 4) {
+                        const float4 x = *reinterpret_cast<const float4*>(s.buf + p + k);
+                        v[k] = seen >> k & 1u ? x.x : v[k];
+                        v[k + 1] = seen >> (k + 1) & 1u ? x.y : v[k + 1];
+                        v[k + 2] = seen >> (k + 2) & 1u ? x.z : v[k + 2];
+                        v[k + 3] = seen >> (k + 3) & 1u ? x.w : v[k + 3];
                     }
+                }
+                if (deny) {
+#pragma unroll
+                    for (uint32_t k = 0; k < N; k++) v[k] = deny >> k & 1u ? -INFINITY : v[k];
                 }
             }
             to(p, v);
@@ -289,17 +311,16 @@ k_adjust(const __grid_constant__ b200bpe_logits in, uint32_t vocab, T* out, uint
     uint4 ahead[SM_AHEAD];
     first_loads(row, s, ahead);
     const MaskRow mask = mask_row(in, s.row);
-    Penalty pen{1.0f, 0.0f, 0.0f};
-    const bool any_special = find_special(in, vocab, s, mask, pen, special);
+    const bool any_special = find_special(in, vocab, row, s, mask, special);
     T* to = out + (uint64_t)s.row * out_stride + s.lo;
     // Places that lie on 16 bytes in the logits do so in the output if its rows are aligned like the logits' (in place, and with equal strides).
     const bool alike = (reinterpret_cast<uint64_t>(to) & 15u) == s.lead * sizeof(T);
     constexpr uint32_t N = Packed<T>::N;
     if (!in.n_bias) {
-        each_adjusted(row, s, ahead, any_special, special, pen, [&](uint32_t p, float (&v)[N]) { write_out<T>(to, s, alike, p, v); });
+        each_adjusted(row, s, ahead, any_special, special, [&](uint32_t p, float (&v)[N]) { write_out<T>(to, s, alike, p, v); });
         return;
     }
-    each_adjusted(row, s, ahead, any_special, special, pen, [&](uint32_t p, float (&v)[N]) { store(buf + p, v); });
+    each_adjusted(row, s, ahead, any_special, special, [&](uint32_t p, float (&v)[N]) { store(buf + p, v); });
     __syncthreads();
     add_biases(in, s, mask);
     __syncthreads();
@@ -896,9 +917,8 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     stats.c = (float)(1.4426950408889634 / set.warm);
     {
         const MaskRow mask = mask_row(in, sl.row);
-        Penalty pen{1.0f, 0.0f, 0.0f};
-        const bool any_special = find_special(in, vocab, sl, mask, pen, s.special);
-        each_adjusted(row, sl, ahead, any_special, s.special, pen, [&](uint32_t p, float (&v)[Packed<T>::N]) {
+        const bool any_special = find_special(in, vocab, row, sl, mask, s.special);
+        each_adjusted(row, sl, ahead, any_special, s.special, [&](uint32_t p, float (&v)[Packed<T>::N]) {
             store(buf + p, v);
             if (!in.n_bias) stats.add(v, p, buf);
         });
@@ -1218,7 +1238,7 @@ using namespace b200bpe;
 extern "C" {
 
 b200bpe_status b200bpe_sampler_create(b200bpe_ctx* c, uint32_t vocab_size, b200bpe_sampler** out) {
-    if (vocab_size == 0 || vocab_size > SM_MAX_VOCAB) return refused("b200bpe_sampler_create: 1 to 524,288 tokens");
+    if (vocab_size == 0 || vocab_size > SM_MAX_VOCAB) return refused("b200bpe_sampler_create: 1 to 327,680 tokens");
     if (!c || !out) return refused("b200bpe_sampler_create: null pointer");
     const OnDevice on(c->c.device);
     B2_CUDA(on.error);

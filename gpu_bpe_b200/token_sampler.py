@@ -31,8 +31,8 @@ class TokenSampler:
     def __init__(self, engine, vocabSize: int):
         self._engine, self.vocabSize = engine, int(vocabSize)
         self._h = None
-        if not 1 <= self.vocabSize <= 524288:
-            raise ValueError("vocabSize: 1 to 524,288 tokens")
+        if not 1 <= self.vocabSize <= 327680:
+            raise ValueError("vocabSize: 1 to 327,680 tokens")
         h = C.c_void_p()
         _lib.check(_lib.lib().b200bpe_sampler_create(engine.ctx, self.vocabSize, C.byref(h)), "b200bpe_sampler_create")
         self._h = h

@@ -332,7 +332,7 @@ typedef struct {
 } b200bpe_choice;
 
 typedef struct b200bpe_sampler b200bpe_sampler;
-/* vocab_size: 1 to 524,288 tokens (a row's x stays on chip, shared out over a cluster's memory). */
+/* vocab_size: 1 to 327,680 tokens (a row's x stays on chip, shared out over a cluster's memory). */
 b200bpe_status b200bpe_sampler_create(b200bpe_ctx*, uint32_t vocab_size, b200bpe_sampler** out);
 /* The x of every row, rounded once to the logits' type.  Columns behind the vocabulary are left as they are. */
 b200bpe_status b200bpe_sampler_adjust(b200bpe_sampler*, const b200bpe_logits*, void* logits_out, uint64_t out_stride, void* stream);

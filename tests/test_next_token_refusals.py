@@ -126,8 +126,8 @@ def test_a_destroyed_handle():
 
 def test_what_makes_no_handle():
     engine = types.SimpleNamespace(ctx=None, device_index=0)
-    for n in (0, -1, 524289):
-        with pytest.raises(ValueError, match="524,288"):
+    for n in (0, -1, 327681):
+        with pytest.raises(ValueError, match="327,680"):
             TokenSampler(engine, n)
     table, ends = np.full((2, 256), -1), [0, 1]
     for arguments, text in [((table[:, :255], ends), "transitions"), ((table.astype(float), ends), "transitions"), ((table, [1]), "accepting"),
@@ -147,8 +147,8 @@ def _refused(status, text):
 def test_c_entry_points():
     """Arguments are looked at before the handles, so that a machine without a GPU can tell."""
     L, h = _lib.lib(), C.c_void_p()
-    _refused(L.b200bpe_sampler_create(None, 0, C.byref(h)), "524,288")
-    _refused(L.b200bpe_sampler_create(None, 524289, C.byref(h)), "524,288")
+    _refused(L.b200bpe_sampler_create(None, 0, C.byref(h)), "327,680")
+    _refused(L.b200bpe_sampler_create(None, 327681, C.byref(h)), "327,680")
     _refused(L.b200bpe_sampler_create(None, 5, C.byref(h)), "null")
     p, c = _lib.Logits(), _lib.Choice()
     p.struct_size, c.struct_size = C.sizeof(_lib.Logits), C.sizeof(_lib.Choice)
