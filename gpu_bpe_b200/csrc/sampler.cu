@@ -410,18 +410,27 @@ constexpr uint32_t SM_QUICK_K = 512;             // top_k up to which a row's ca
 // w = 2^(x c - n) with c = log2 e / temperature, and added in 64 bits.  Against the exact weights, up to a factor that all have in common, the
 // exponent is off by the roundings of c and of the product's difference, together 2 * 2^-24 (m - x) c + 2^-24, the exponential by 2^-22 of itself, and up to
 // eight weights are added in 32 bits first, three roundings: a sum is off by at most
-//     E = sum w * 2^-24 * (8 + 2 ln 2 (m - x) c).
+//     E = sum w * 2^-24 * (10 + 2 ln 2 (m - x) c),
+// with two for the factor that brings such sums to the unit of the others, where that matters.
 // The mean of (m - x) c under the weights is their entropy less log2 Z, Z = sum w / max w, so at most log2(tokens / Z).  A border that is a share u of
 // the sum S has its part of the same errors: a running sum s is off from u S by (1 - u) times what s is off less u times what the rest is off, less than
 // E.  Where a running sum that decides lies within E of the border, the row's sums are made again of weights in 64 bits.
 struct Weights {
-    float m, c, n;      // the largest x, log2 e / temperature, the exponent that all weights are relative to
-    double by;          // 1 / temperature
+    float m, c, n;              // the largest x, log2 e / temperature, the exponent that all quick weights are relative to
+    double steps;               // 64 log2 e / temperature
+    const double* table;        // 2^(i / 64)
     __device__ __forceinline__ float quick(float x) const { return Stats::two_to(fmaf(x, c, -n)); }
-    // relative to the largest
-    __device__ __forceinline__ double log_of(float x) const { return ((double)x - (double)m) * by; }
-    __device__ __forceinline__ double exact(float x) const { return exp(log_of(x)); }
-    __device__ __forceinline__ double to_largest() const { return exp2((double)n - (double)m * (double)c); }        // quick's unit in exact's
+    // e^((x - m) / temperature) = 2^(t / 64) with t = k + r, |r| <= 1/2: a table's value, the first five terms of the series for r (the sixth is below
+    // 4e-14), and a power of two; 11 operations in 64 bits.  Of m itself it is 1.
+    __device__ __forceinline__ double exact(float x) const {
+        constexpr double MAGIC = 6755399441055744.0, L = 0.693147180559945309 / 64;
+        const double t = ((double)x - (double)m) * steps, u = t + MAGIC, r = t - (u - MAGIC);
+        const int k = __double2loint(u);
+        const double p = table[k & 63] * fma(r, fma(r, fma(r, fma(r, L * L * L * L / 24, L * L * L / 6), L * L / 2), L), 1.0);
+        return fmaf(x, c, -n) > -1000.0f ? __hiloint2double(__double2hiint(p) + (k >> 6) * 1048576, __double2loint(p)) : 0.0;
+    }
+    __device__ __forceinline__ double power_of_largest() const { return (double)n - (double)m * (double)c; }
+    __device__ __forceinline__ double to_largest() const { return (double)exp2f((float)power_of_largest()); }        // quick's unit in exact's
 };
 
 // What of the row is kept: x with a larger key, and those with the key in front of token `end`.
@@ -438,7 +447,7 @@ struct Best { float m, n; uint32_t at, pad; double sum; float cut[4]; };       /
 struct Shared {
     Best best[SM_MAX_CLUSTER];
     double part_warp[2][SM_WARPS], part_cta[2][2][SM_MAX_CLUSTER];      // (the second index: one exchange and the next)
-    double scan_warp[SM_WARPS], warp_mass[SM_WARPS];
+    double scan_warp[SM_WARPS], warp_mass[SM_WARPS], table[64];
     float m_warp[SM_WARPS], n_warp[SM_WARPS], cut[4];
     uint32_t border[2], candidates, quick_candidates, flag, place, at, cut_at[2];
     Kept kept;
@@ -561,45 +570,70 @@ __device__ uint32_t find_place(Team& t, const Slice& sl, double base, double tar
         for (int w = 0; w < owner; w++) at += s.warp_mass[w];
     }
     if (t.warp == owner) {
+        // the sums of steps of 128 places, 32 steps at a time, then the step that passes the target
         const Span span(sl.padded, t.warp);
         uint32_t place = 0;
         bool close = false, found = false;
-        for (uint32_t p0 = span.lo; p0 < span.hi && !found; p0 += 128) {
-            const uint32_t p = p0 + t.lane * 4;
-            double v[4] = {0, 0, 0, 0};
-            if (p < span.hi) {
-                const float4 x = *reinterpret_cast<const float4*>(sl.buf + p);
-                v[0] = f(p, x.x); v[1] = f(p + 1, x.y); v[2] = f(p + 2, x.z); v[3] = f(p + 3, x.w);
+        const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        for (uint32_t p0 = span.lo; p0 < span.hi && !found; p0 += 32 * 128) {
+            const int steps = (int)min(32u, (span.hi - p0 + 127u) / 128u);
+            double step_sum = 0;
+#pragma unroll 4
+            for (int i = 0; i < steps; i++) {
+                const uint32_t p = p0 + i * 128 + t.lane * 4;
+                const float4 x = p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : nothing;
+                double v = (f(p, x.x) + f(p + 1, x.y)) + (f(p + 2, x.z) + f(p + 3, x.w));
+#pragma unroll
+                for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+                if (t.lane == i) step_sum = v;
             }
-            const double mine = (v[0] + v[1]) + (v[2] + v[3]);
-            double run = mine;
+            double run = step_sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const double y = __shfl_up_sync(0xFFFFFFFFu, run, o);
                 if (t.lane >= o) run += y;
             }
-            double sum = at + run - mine;
-            uint32_t hit = 0, last = 0;
-            bool edge = false;
-            for (int k = 3; k >= 0; k--) if (v[k] > 0 && last == 0) last = p + k + 1;
-            for (int k = 0; k < 4; k++) {
-                const double next = sum + v[k];
-                if (v[k] > 0 && hit == 0) {
-                    edge = fabs(next - target) <= margin || fabs(sum - target) <= margin;
-                    if (next > target) hit = p + k + 1;
+            // (behind the first step above the target, and in front of it where rounding has it, there are others to look at)
+            uint32_t todo = __ballot_sync(0xFFFFFFFFu, step_sum > 0 && at + run > target);
+            const uint32_t filled_steps = __ballot_sync(0xFFFFFFFFu, step_sum > 0);
+            const bool any = todo != 0;
+            if (!any && filled_steps) todo = 1u << (31 - __clz(filled_steps));
+            if (todo) {
+                const int i = __ffs(todo) - 1;
+                const uint32_t p = p0 + i * 128 + t.lane * 4;
+                const float4 x = p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : nothing;
+                const double v[4] = {f(p, x.x), f(p + 1, x.y), f(p + 2, x.z), f(p + 3, x.w)}, mine = (v[0] + v[1]) + (v[2] + v[3]);
+                double sum = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const double y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+                    if (t.lane >= o) sum += y;
                 }
-                sum = next;
+                sum += at + __shfl_sync(0xFFFFFFFFu, run - step_sum, i) - mine;
+                uint32_t hit = 0, last = 0;
+                bool edge = false;
+                for (int k = 3; k >= 0; k--) if (v[k] > 0 && last == 0) last = p + k + 1;
+                for (int k = 0; k < 4; k++) {
+                    const double next = sum + v[k];
+                    if (v[k] > 0 && hit == 0) {
+                        edge = fabs(next - target) <= margin || fabs(sum - target) <= margin;
+                        if (next > target) hit = p + k + 1;
+                    }
+                    sum = next;
+                }
+                const uint32_t above = __ballot_sync(0xFFFFFFFFu, hit != 0), some = __ballot_sync(0xFFFFFFFFu, last != 0);
+                if (above && any) {
+                    const int l = __ffs(above) - 1;
+                    place = __shfl_sync(0xFFFFFFFFu, hit, l) - 1;
+                    close = __shfl_sync(0xFFFFFFFFu, edge, l);
+                    found = true;
+                } else if (some) {       // the last one there is; in 64 bits, the sum of a step and the running one may round apart
+                    place = __shfl_sync(0xFFFFFFFFu, last, 31 - __clz(some)) - 1;
+                    found = any;
+                    close = true;
+                }
             }
-            const uint32_t above = __ballot_sync(0xFFFFFFFFu, hit != 0), some = __ballot_sync(0xFFFFFFFFu, last != 0);
-            if (above) {
-                const int l = __ffs(above) - 1;
-                place = __shfl_sync(0xFFFFFFFFu, hit, l) - 1;
-                close = __shfl_sync(0xFFFFFFFFu, edge, l);
-                found = true;
-            } else {
-                if (some) place = __shfl_sync(0xFFFFFFFFu, last, 31 - __clz(some)) - 1;
-                at += __shfl_sync(0xFFFFFFFFu, run, 31);
-            }
+            at += __shfl_sync(0xFFFFFFFFu, run, 31);
         }
         // (no sum above the target: only where rounding, or a uniform of 1, put the target at the whole sum)
         if (t.lane == 0) { s.place = place; s.flag = close || !found; }
@@ -934,21 +968,16 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     float m, n;
     double all;
     for (bool again = false;; again = true) {
-        m = stats.m;
-        n = stats.n;
-        double sum = stats.sum;
+        m = value_of(__reduce_max_sync(0xFFFFFFFFu, key_of(stats.m)));
+        n = stats.base(m);
+        double sum = stats.sum * Stats::power(stats.n - n);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            const float to = fmaxf(n, __shfl_xor_sync(0xFFFFFFFFu, n, o));
-            sum *= Stats::power(n - to);
-            sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-            n = to;
-            m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        }
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         __syncthreads();
         if (t.lane == 0) { s.m_warp[t.warp] = m; s.n_warp[t.warp] = n; s.part_warp[0][t.warp] = sum; }
         if (threadIdx.x == 0) { s.at = 0xFFFFFFFFu; s.quick_candidates = 0u; }
         if (threadIdx.x < 4) s.cut[threadIdx.x] = -INFINITY;
+        if (threadIdx.x < 64 && !set.greedy) s.table[threadIdx.x] = exp2((double)threadIdx.x / 64);
         if (quick_k) s.keys[threadIdx.x] = key_of(stats.m);
         else if (by_k || by_p)
             for (uint32_t i = threadIdx.x; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0u;
@@ -998,14 +1027,15 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         }
         return;
     }
-    const Weights w{m, stats.c, n, 1.0 / set.warm};
+    const Weights w{m, stats.c, n, 64 * 1.4426950408889634 / set.warm, s.table};
     const double unit = w.to_largest();
     all = 0;
     for (uint32_t c = 0; c < t.C; c++) all += s.best[c].sum * Stats::power(s.best[c].n - n);
-    all *= unit;
+    const double quick_all = all;
     auto answer = [&](uint32_t token, float x) {
         how.tokens_out[sl.row] = token;
-        if (how.logprobs_out) how.logprobs_out[sl.row] = (float)(w.log_of(x) - log(all));
+        if (how.logprobs_out)
+            how.logprobs_out[sl.row] = (float)(((double)x - (double)m) / set.warm - (log(quick_all) + 0.693147180559945309 * w.power_of_largest()));
     };
     if (set.greedy) {
         if (t.rank == 0 && threadIdx.x == 0) {
@@ -1016,7 +1046,8 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         }
         return;
     }
-    const double margin = all * (8.0 + 1.4 * (log2((double)vocab / all) + 1.0)) / 16777216.0;
+    all *= unit;
+    const double margin = all * (double)((10.0f + 1.4f * (log2f((float)vocab / (float)all) + 1.0f)) / 16777216.0f);
 
     // The kept tokens.
     Kept kept{LOWEST_KEY, 0u};
