@@ -447,7 +447,7 @@ struct Best { float m, n; uint32_t at, pad; double sum; float cut[4]; };       /
 struct Shared {
     Best best[SM_MAX_CLUSTER];
     double part_warp[2][SM_WARPS], part_cta[2][2][SM_MAX_CLUSTER];      // (the second index: one exchange and the next)
-    double scan_warp[SM_WARPS], warp_mass[SM_WARPS], table[64];
+    double scan_warp[SM_WARPS], warp_mass[SM_WARPS], step_mass[32], table[64];
     float m_warp[SM_WARPS], n_warp[SM_WARPS], cut[4];
     uint32_t border[2], candidates, quick_candidates, flag, place, at, cut_at[2];
     Kept kept;
@@ -458,6 +458,20 @@ struct Shared {
         Special<SM_MAX_SLICE + 8> special;           // until the slice is there
     };
 };
+
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ double warp_run(double v, int lane) {        // over the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += y;
+    }
+    return v;
+}
 
 // One CTA's view of its cluster.
 struct Team {
@@ -479,39 +493,30 @@ struct Team {
     // Sums of two values over the cluster; every CTA's part of them stays in part(i, cta) until the exchange after the next, every warp's part of
     // the first in s.warp_mass until the next.
     __device__ void total(double& a, double& b) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1) {
-            a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
-            b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
-        }
+        a = warp_sum(a);
+        b = warp_sum(b);
         __syncthreads();
         if (lane == 0) { s.part_warp[0][warp] = s.warp_mass[warp] = a; s.part_warp[1][warp] = b; }
         __syncthreads();
         par ^= 1;
         if (warp == 0) {
-            a = b = 0;
-#pragma unroll
-            for (int w = 0; w < SM_WARPS; w++) { a += s.part_warp[0][w]; b += s.part_warp[1][w]; }
-            if (threadIdx.x < C) {
-                Shared* p = peer(threadIdx.x);
+            a = warp_sum(lane < SM_WARPS ? s.part_warp[0][lane] : 0.0);
+            b = warp_sum(lane < SM_WARPS ? s.part_warp[1][lane] : 0.0);
+            if (lane < C) {
+                Shared* p = peer(lane);
                 p->part_cta[0][par][rank] = a;
                 p->part_cta[1][par][rank] = b;
             }
         }
         sync();
-        a = b = 0;
-        for (uint32_t c = 0; c < C; c++) { a += part(0, c); b += part(1, c); }
+        a = warp_sum(lane < C ? part(0, lane) : 0.0);
+        b = warp_sum(lane < C ? part(1, lane) : 0.0);
     }
     __device__ double part(int i, uint32_t cta) const { return s.part_cta[i][par][cta]; }
 
     // Sum of v over the threads before this one; *all: over all.
     __device__ double before(double v, double* all) {
-        double run = v;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xFFFFFFFFu, run, o);
-            if (lane >= o) run += y;
-        }
+        const double run = warp_run(v, lane);
         __syncthreads();
         if (lane == 31) s.scan_warp[warp] = run;
         __syncthreads();
@@ -523,6 +528,14 @@ struct Team {
         }
         *all = sum;
         return base + run - v;
+    }
+    // The first of n values (a lane's is v) at which the running sum is above target, and the sum in front of it; if there is none, the last above 0.
+    __device__ int first_above(double v, double from, double target, double* base) const {
+        const double run = from + warp_run(v, lane);
+        const uint32_t above = __ballot_sync(0xFFFFFFFFu, v > 0 && run > target), some = __ballot_sync(0xFFFFFFFFu, v > 0);
+        const int i = above ? __ffs(above) - 1 : some ? 31 - __clz(some) : 0;
+        *base = __shfl_sync(0xFFFFFFFFu, run - v, i);
+        return i;
     }
 };
 
@@ -553,90 +566,53 @@ __device__ __forceinline__ double kept_mass(const Slice& sl, int warp, const Wei
 }
 
 // The first place of the slice at which base plus the running sum of f(place, x) is above target; if there is none, the last with f above 0.  Every
-// warp's sum of f is in s.warp_mass.  *near: whether a sum that decided was within `margin` of target.  Called by all threads of one CTA.
+// warp's sum of f is in s.warp_mass.  *near: whether a sum that decided was within `margin` of target (or the sums of parts and of places round apart).
+// Called by all threads of one CTA: first the part of a warp, then a step of 128 places of it, then a place.
 template <class F>
 __device__ uint32_t find_place(Team& t, const Slice& sl, double base, double target, double margin, bool* near, F f) {
+    static_assert(SM_MAX_SLICE + 8 <= SM_WARPS * 32 * 128, "more than 32 steps in a warp's part");
     Shared& s = t.s;
-    double at = base;
-    int owner = -1, filled = 0;
-    for (int w = 0; w < SM_WARPS && owner < 0; w++) {
-        if (s.warp_mass[w] > 0) filled = w;
-        if (at + s.warp_mass[w] > target) owner = w;
-        else at += s.warp_mass[w];
-    }
-    if (owner < 0) {
-        owner = filled;
-        at = base;
-        for (int w = 0; w < owner; w++) at += s.warp_mass[w];
-    }
-    if (t.warp == owner) {
-        // the sums of steps of 128 places, 32 steps at a time, then the step that passes the target
-        const Span span(sl.padded, t.warp);
-        uint32_t place = 0;
-        bool close = false, found = false;
-        const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-        for (uint32_t p0 = span.lo; p0 < span.hi && !found; p0 += 32 * 128) {
-            const int steps = (int)min(32u, (span.hi - p0 + 127u) / 128u);
-            double step_sum = 0;
-#pragma unroll 4
-            for (int i = 0; i < steps; i++) {
-                const uint32_t p = p0 + i * 128 + t.lane * 4;
-                const float4 x = p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : nothing;
-                double v = (f(p, x.x) + f(p + 1, x.y)) + (f(p + 2, x.z) + f(p + 3, x.w));
-#pragma unroll
-                for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-                if (t.lane == i) step_sum = v;
-            }
-            double run = step_sum;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xFFFFFFFFu, run, o);
-                if (t.lane >= o) run += y;
-            }
-            // (behind the first step above the target, and in front of it where rounding has it, there are others to look at)
-            uint32_t todo = __ballot_sync(0xFFFFFFFFu, step_sum > 0 && at + run > target);
-            const uint32_t filled_steps = __ballot_sync(0xFFFFFFFFu, step_sum > 0);
-            const bool any = todo != 0;
-            if (!any && filled_steps) todo = 1u << (31 - __clz(filled_steps));
-            if (todo) {
-                const int i = __ffs(todo) - 1;
-                const uint32_t p = p0 + i * 128 + t.lane * 4;
-                const float4 x = p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : nothing;
-                const double v[4] = {f(p, x.x), f(p + 1, x.y), f(p + 2, x.z), f(p + 3, x.w)}, mine = (v[0] + v[1]) + (v[2] + v[3]);
-                double sum = mine;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-                    if (t.lane >= o) sum += y;
-                }
-                sum += at + __shfl_sync(0xFFFFFFFFu, run - step_sum, i) - mine;
-                uint32_t hit = 0, last = 0;
-                bool edge = false;
-                for (int k = 3; k >= 0; k--) if (v[k] > 0 && last == 0) last = p + k + 1;
-                for (int k = 0; k < 4; k++) {
-                    const double next = sum + v[k];
-                    if (v[k] > 0 && hit == 0) {
-                        edge = fabs(next - target) <= margin || fabs(sum - target) <= margin;
-                        if (next > target) hit = p + k + 1;
-                    }
-                    sum = next;
-                }
-                const uint32_t above = __ballot_sync(0xFFFFFFFFu, hit != 0), some = __ballot_sync(0xFFFFFFFFu, last != 0);
-                if (above && any) {
-                    const int l = __ffs(above) - 1;
-                    place = __shfl_sync(0xFFFFFFFFu, hit, l) - 1;
-                    close = __shfl_sync(0xFFFFFFFFu, edge, l);
-                    found = true;
-                } else if (some) {       // the last one there is; in 64 bits, the sum of a step and the running one may round apart
-                    place = __shfl_sync(0xFFFFFFFFu, last, 31 - __clz(some)) - 1;
-                    found = any;
-                    close = true;
-                }
-            }
-            at += __shfl_sync(0xFFFFFFFFu, run, 31);
+    const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    const Span span(sl.padded, t.first_above(t.lane < SM_WARPS ? s.warp_mass[t.lane] : 0.0, base, target, &base));
+    for (uint32_t i = t.warp; i < 32; i += SM_WARPS) {
+        const uint32_t p = span.lo + i * 128 + t.lane * 4;
+        double v = 0;
+        if (span.lo + i * 128 < span.hi) {
+            const float4 x = p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : nothing;
+            v = warp_sum((f(p, x.x) + f(p + 1, x.y)) + (f(p + 2, x.z) + f(p + 3, x.w)));
         }
-        // (no sum above the target: only where rounding, or a uniform of 1, put the target at the whole sum)
-        if (t.lane == 0) { s.place = place; s.flag = close || !found; }
+        if (t.lane == 0) s.step_mass[i] = v;
+    }
+    __syncthreads();
+    if (t.warp == 0) {
+        const int step = t.first_above(s.step_mass[t.lane], base, target, &base);
+        const uint32_t p = span.lo + step * 128 + t.lane * 4;
+        const float4 x = p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : nothing;
+        const double v[4] = {f(p, x.x), f(p + 1, x.y), f(p + 2, x.z), f(p + 3, x.w)}, mine = (v[0] + v[1]) + (v[2] + v[3]);
+        double sum = base + warp_run(mine, t.lane) - mine;
+        uint32_t hit = 0, last = 0;
+        bool edge = false;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const double next = sum + v[k];
+            if (v[k] > 0) {
+                last = p + k + 1;
+                if (hit == 0) {
+                    edge = fabs(next - target) <= margin || fabs(sum - target) <= margin;
+                    if (next > target) hit = p + k + 1;
+                }
+            }
+            sum = next;
+        }
+        const uint32_t above = __ballot_sync(0xFFFFFFFFu, hit != 0), some = __ballot_sync(0xFFFFFFFFu, last != 0);
+        const int l = above ? __ffs(above) - 1 : some ? 31 - __clz(some) : 0;
+        hit = __shfl_sync(0xFFFFFFFFu, hit, l);
+        last = __shfl_sync(0xFFFFFFFFu, last, l);
+        edge = __shfl_sync(0xFFFFFFFFu, edge, l);
+        if (t.lane == 0) {
+            s.place = (above ? hit : some ? last : 1u) - 1u;
+            s.flag = edge || !above;
+        }
     }
     __syncthreads();
     *near = s.flag != 0;
@@ -670,8 +646,8 @@ struct Bins {
     }
 };
 
-// Appends a lane's values whose bits are set in `in`, of tokens from v0 on, to the list of the cluster's first CTA, as far as there is room.
-__device__ __forceinline__ void gather(Team& t, uint32_t* counter, unsigned long long* list, const float (&v)[4], uint32_t in, uint32_t v0) {
+// Appends a lane's values whose bits are set in `in`, of tokens from v0 on, to a list, as far as there is room.
+__device__ __forceinline__ void gather(const Team& t, uint32_t* counter, unsigned long long* list, const float (&v)[4], uint32_t in, uint32_t v0) {
     if (!__any_sync(0xFFFFFFFFu, in != 0u)) return;
     uint32_t before = 0, all = 0;
 #pragma unroll
@@ -689,6 +665,19 @@ __device__ __forceinline__ void gather(Team& t, uint32_t* counter, unsigned long
             if (base < SM_CANDIDATES) list[base] = (unsigned long long)key_of(v[k]) << 32 | (uint32_t)~(v0 + k);
             base++;
         }
+}
+// The candidates of a CTA other than the first, gathered in its own list, go to the first one's: a CTA waits once for the way there and back.  The
+// cluster's next barrier makes them seen.
+__device__ __forceinline__ void hand_over(Team& t, uint32_t Shared::*counter) {
+    Shared& s = t.s;
+    if (t.rank == 0) return;
+    __syncthreads();
+    const uint32_t n = s.*counter;
+    if (n == 0) return;
+    Shared* lead = t.peer(0);
+    if (threadIdx.x == 0) s.place = atomicAdd(&(lead->*counter), n);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < min(n, SM_CANDIDATES) && s.place + i < SM_CANDIDATES; i += SM_THREADS) lead->list[s.place + i] = s.list[i];
 }
 
 // The part of the row's order at which a running sum, from the largest x on, reaches `target`: of weights (MASS) or of tokens.
@@ -736,7 +725,6 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     // sums of what is above the border's bins; what lies in them goes to the first CTA
     const uint32_t from = s.border[0], to = max(s.border[1], from);
     double above = 0, count = 0;
-    Shared* lead = t.peer(0);
     each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
         const float v[4] = {x.x, x.y, x.z, x.w};
         float part = 0;
@@ -748,9 +736,9 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
             else if (b <= to && v[k] > -INFINITY) in |= 1u << k;
         }
         above += (double)part;
-        // (the list lies where the first CTA's bins were)
-        gather(t, &lead->candidates, lead->list, v, in, p + shift);
+        gather(t, &s.candidates, s.list, v, in, p + shift);      // (the list lies where the bins were)
     });
+    hand_over(t, &Shared::candidates);
     if (MASS) above *= w.to_largest();
     t.total(above, count);
     const uint32_t n = t.peer(0)->candidates;
@@ -844,9 +832,8 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     });
     t.total(equal, none);
     if (ties >= equal) return Kept{low, 0xFFFFFFFFu};
-    double base = 0;
-    uint32_t owner = 0;
-    while (owner + 1 < t.C && base + t.part(0, owner) < ties) base += t.part(0, owner++);
+    double base;
+    const uint32_t owner = t.first_above(t.lane < t.C ? t.part(0, t.lane) : 0.0, 0.0, ties - 0.5, &base);
     if (t.rank == owner) {
         bool near;
         const uint32_t p = find_place(t, sl, base, ties - 0.5, 0.0, &near, [&](uint32_t, float x) { return key_of(x) == low ? 1.0 : 0.0; });
@@ -888,10 +875,12 @@ __device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& 
     __syncthreads();
     sort_down(s.list, size);
     n = min(n, set.top_k);
-    const uint32_t i0 = threadIdx.x * SM_EACH, min_key = set.min_key(w.m);
+    // neighbours to a thread
+    const uint32_t each = max(size / SM_THREADS, 1u), i0 = threadIdx.x * each, min_key = set.min_key(w.m);
     double v[SM_EACH], mine = 0, all;
+#pragma unroll
     for (uint32_t k = 0; k < SM_EACH; k++) {
-        v[k] = i0 + k < n ? w.exact(value_of((uint32_t)(s.list[i0 + k] >> 32))) : 0.0;
+        v[k] = k < each && i0 + k < n ? w.exact(value_of((uint32_t)(s.list[i0 + k] >> 32))) : 0.0;
         mine += v[k];
     }
     if (threadIdx.x == 0) s.place = 0u;
@@ -899,21 +888,26 @@ __device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& 
     const double enough = (double)set.top_p * all;
     // what stays, with the token in front, so that the order becomes the tokens'
     unsigned long long e[SM_EACH];
+#pragma unroll
     for (uint32_t k = 0; k < SM_EACH; k++) {
-        const unsigned long long c = i0 + k < n ? s.list[i0 + k] : 0ull;
-        const bool stays = i0 + k < n && (set.top_p >= 1.0f || sum < enough || i0 + k == 0u) && (uint32_t)(c >> 32) >= min_key;
+        const unsigned long long c = k < each && i0 + k < n ? s.list[i0 + k] : 0ull;
+        const bool stays = c && (set.top_p >= 1.0f || sum < enough || i0 + k == 0u) && (uint32_t)(c >> 32) >= min_key;
         e[k] = stays ? c << 32 | c >> 32 : 0ull;
         sum += v[k];
     }
     __syncthreads();
+#pragma unroll
     for (uint32_t k = 0; k < SM_EACH; k++)
-        if (i0 + k < size) s.list[i0 + k] = e[k];
+        if (k < each && i0 + k < size) s.list[i0 + k] = e[k];
     __syncthreads();
+    size = 2;
+    while (size < n) size *= 2;              // (the first n, in the order of x, were looked at)
     sort_down(s.list, size);
     mine = 0;
     uint32_t filled = 0;
+#pragma unroll
     for (uint32_t k = 0; k < SM_EACH; k++) {
-        const unsigned long long c = i0 + k < size ? s.list[i0 + k] : 0ull;
+        const unsigned long long c = k < each && i0 + k < size ? s.list[i0 + k] : 0ull;
         v[k] = c ? w.exact(value_of((uint32_t)c)) : 0.0;
         if (v[k] > 0) filled = i0 + k;
         mine += v[k];
@@ -922,6 +916,7 @@ __device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& 
     sum = t.before(mine, &all);
     const double target = (double)set.uniform * all;
     __syncthreads();
+#pragma unroll
     for (uint32_t k = 0; k < SM_EACH; k++) {
         if (v[k] > 0 && sum <= target && sum + v[k] > target) s.place = i0 + k;
         sum += v[k];
@@ -971,8 +966,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         m = value_of(__reduce_max_sync(0xFFFFFFFFu, key_of(stats.m)));
         n = stats.base(m);
         double sum = stats.sum * Stats::power(stats.n - n);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        sum = warp_sum(sum);
         __syncthreads();
         if (t.lane == 0) { s.m_warp[t.warp] = m; s.n_warp[t.warp] = n; s.part_warp[0][t.warp] = sum; }
         if (threadIdx.x == 0) { s.at = 0xFFFFFFFFu; s.quick_candidates = 0u; }
@@ -982,34 +976,37 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         else if (by_k || by_p)
             for (uint32_t i = threadIdx.x; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0u;
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < SM_WARPS; i++) { m = fmaxf(m, s.m_warp[i]); n = fmaxf(n, s.n_warp[i]); }
+        m = value_of(__reduce_max_sync(0xFFFFFFFFu, key_of(s.m_warp[t.lane % SM_WARPS])));
+        n = stats.base(m);
         if (stats.m == m && m > -INFINITY) {
             uint32_t p = stats.at;
             while (buf[p] != m) p++;
             atomicMin(&s.at, p + shift);
         }
-        if (quick_k) {
-            uint32_t rank = 0;
-            const uint32_t mine = key_of(stats.m);
-            for (uint32_t i = 0; i < SM_THREADS; i += 4) {
-                const uint4 k = *reinterpret_cast<const uint4*>(s.keys + i);
-                rank += (k.x > mine || (k.x == mine && i < threadIdx.x)) + (k.y > mine || (k.y == mine && i + 1 < threadIdx.x)) +
-                        (k.z > mine || (k.z == mine && i + 2 < threadIdx.x)) + (k.w > mine || (k.w == mine && i + 3 < threadIdx.x));
+        if (quick_k && t.warp < 4) {
+            // cut[l]: at least top_k / 2^l of this slice are not below it.  The largest keys by their upper half that so many threads' largest x have.
+            const uint32_t wanted = (set.top_k + (1u << t.warp) - 1u) >> t.warp;
+            uint32_t k[SM_THREADS / 32], cut = 0u;
+#pragma unroll
+            for (int i = 0; i < SM_THREADS / 32; i++) k[i] = s.keys[i * 32 + t.lane] >> 16;
+            for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+                uint32_t so_many = 0;
+#pragma unroll
+                for (int i = 0; i < SM_THREADS / 32; i++) so_many += k[i] >= (cut | bit);
+                if (__reduce_add_sync(0xFFFFFFFFu, so_many) >= wanted) cut |= bit;
             }
-            // cut[l]: at least top_k / 2^l of this slice are not below it
-            for (int l = 0; l < 4; l++)
-                if (rank + 1u == (set.top_k + (1u << l) - 1u) >> l) s.cut[l] = stats.m;
+            if (t.lane == 0 && cut > LOWEST_KEY >> 16) s.cut[t.warp] = value_of(cut << 16);
         }
         __syncthreads();
         if (!again) cluster.barrier_wait();
-        if (threadIdx.x < t.C) {
-            Best b{m, n, s.at, 0u, 0.0, {s.cut[0], s.cut[1], s.cut[2], s.cut[3]}};
-            for (int i = 0; i < SM_WARPS; i++) b.sum += s.part_warp[0][i] * Stats::power(s.n_warp[i] - n);
-            t.peer(threadIdx.x)->best[t.rank] = b;
+        if (t.warp == 0) {
+            const Best b{m, n, s.at, 0u, warp_sum(t.lane < SM_WARPS ? s.part_warp[0][t.lane] * Stats::power(s.n_warp[t.lane] - n) : 0.0),
+                         {s.cut[0], s.cut[1], s.cut[2], s.cut[3]}};
+            if (t.lane < t.C) t.peer(t.lane)->best[t.rank] = b;
         }
         t.sync();
-        for (uint32_t c = 0; c < t.C; c++) { m = fmaxf(m, s.best[c].m); n = fmaxf(n, s.best[c].n); }
+        m = value_of(__reduce_max_sync(0xFFFFFFFFu, t.lane < t.C ? key_of(s.best[t.lane].m) : LOWEST_KEY));
+        n = stats.base(m);
         if (again || m == -INFINITY || fabsf(m) * stats.c < Stats::FAR) break;
         // So far out that only differences from m mean something.
         for (uint32_t p = threadIdx.x; p < sl.padded; p += SM_THREADS) buf[p] = buf[p] == m ? 0.0f : m == INFINITY ? -INFINITY : buf[p] - m;
@@ -1029,8 +1026,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     }
     const Weights w{m, stats.c, n, 64 * 1.4426950408889634 / set.warm, s.table};
     const double unit = w.to_largest();
-    all = 0;
-    for (uint32_t c = 0; c < t.C; c++) all += s.best[c].sum * Stats::power(s.best[c].n - n);
+    all = warp_sum(t.lane < t.C ? s.best[t.lane].sum * Stats::power(s.best[t.lane].n - n) : 0.0);
     const double quick_all = all;
     auto answer = [&](uint32_t token, float x) {
         how.tokens_out[sl.row] = token;
@@ -1073,8 +1069,9 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
             uint32_t in = 0;
 #pragma unroll
             for (int k = 0; k < 4; k++) in |= (uint32_t)(v[k] >= from && v[k] > -INFINITY) << k;
-            gather(t, &lead->quick_candidates, lead->list, v, in, p + shift);
+            gather(t, &s.quick_candidates, s.list, v, in, p + shift);
         });
+        hand_over(t, &Shared::quick_candidates);
         t.sync();
         const uint32_t so_many = lead->quick_candidates;
         cluster.barrier_arrive();
@@ -1153,20 +1150,9 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
             double mass = kept_mass<EXACT>(sl, t.warp, w, kept), none = 0;
             t.total(mass, none);
         }
-        double mass = 0, base = 0;
-        for (uint32_t c = 0; c < t.C; c++) mass += t.part(0, c);
-        const double target = (double)set.uniform * mass;
-        uint32_t owner = 0xFFFFFFFFu, filled = 0;
-        for (uint32_t c = 0; c < t.C && owner == 0xFFFFFFFFu; c++) {
-            if (t.part(0, c) > 0) filled = c;
-            if (base + t.part(0, c) > target) owner = c;
-            else base += t.part(0, c);
-        }
-        if (owner == 0xFFFFFFFFu) {
-            owner = filled;
-            base = 0;
-            for (uint32_t c = 0; c < owner; c++) base += t.part(0, c);
-        }
+        const double here = t.lane < t.C ? t.part(0, t.lane) : 0.0, target = (double)set.uniform * warp_sum(here);
+        double base;
+        const uint32_t owner = t.first_above(here, 0.0, target, &base);
         if (t.rank == owner) {
             bool near;
             *place = find_place(t, sl, base, target, EXACT ? 0.0 : margin, &near, [&](uint32_t p, float x) {
