@@ -442,6 +442,8 @@ struct Kept {
     }
 };
 
+// Where a draw falls: in which CTA's slice, what is in front of that, and the sum to be passed.
+struct Draw { uint32_t owner; double base, target; };      // (owner 0xFFFFFFFF: not known)
 struct Best { float m, n; uint32_t at, pad; double sum; float cut[4]; };       // a CTA's part of what the first exchange brings
 
 struct Shared {
@@ -449,8 +451,9 @@ struct Shared {
     double part_warp[2][SM_WARPS], part_cta[2][2][SM_MAX_CLUSTER];      // (the second index: one exchange and the next)
     double scan_warp[SM_WARPS], warp_mass[SM_WARPS], step_mass[32], table[64];
     float m_warp[SM_WARPS], n_warp[SM_WARPS], cut[4];
-    uint32_t border[2], candidates, quick_candidates, flag, place, at, cut_at[2];
+    uint32_t border[2], again, candidates, quick_candidates, flag, place, at, cut_at[2];
     Kept kept;
+    Draw draw;
     union {
         uint32_t bins[SM_BINS];
         unsigned long long list[SM_CANDIDATES];      // candidates: key << 32 | ~token
@@ -624,7 +627,7 @@ __device__ void sort_down(unsigned long long* a, uint32_t n) {
     for (uint32_t size = 2; size <= n; size <<= 1)
         for (uint32_t step = size >> 1; step; step >>= 1) {
             for (uint32_t i = threadIdx.x; i < n / 2; i += SM_THREADS) {
-                const uint32_t lo = (i / step) * step * 2 + i % step, hi = lo + step;
+                const uint32_t lo = (i & ~(step - 1u)) << 1 | (i & (step - 1u)), hi = lo + step;
                 const unsigned long long x = a[lo], y = a[hi];
                 if ((x < y) == ((lo & size) == 0)) { a[lo] = y; a[hi] = x; }
             }
@@ -636,13 +639,25 @@ __device__ void sort_down(unsigned long long* a, uint32_t n) {
 struct Bins {
     float m, scale;
     __device__ Bins(float largest, double range) : m(largest), scale((float)(SM_BINS / fmin(range, 3.4e38))) {}
-    static __device__ __forceinline__ uint32_t whole(float x) { return __float_as_uint(x + 8388608.0f) & 0x7FFFFFu; }        // of 0 to 2^22, to the nearest
-    __device__ __forceinline__ float at(float x) const { return fminf((m - x) * scale, (float)(SM_BINS - 1)); }
-    __device__ __forceinline__ uint32_t of(float x) const { return whole(at(x)); }
-    // The weight of what lies at `at`, in parts of 2^16 of the middle of its bin, where a bin is 1/64 wide: e^-r by its first terms.
-    static __device__ __forceinline__ uint32_t weight(float at, uint32_t bin) {
-        const float r = at - (float)bin;
-        return whole(fmaf(fmaf(r, 8.0f, -1024.0f), r, 65536.0f));
+    static constexpr float MAGIC = 8388608.0f;       // added to 0 to 2^22, it leaves the nearest whole number in the lowest bits
+    __device__ __forceinline__ float at(float x) const { return (m - x) * scale; }
+    // Puts x into its bin, if it lies in front of `end`: as 1, or as its weight in parts of 2^16 of that of its bin's middle, bins being 1/64 wide: e^-r by
+    // its first terms.
+    template <bool MASS>
+    __device__ __forceinline__ void put(uint32_t* bins, float x, float end) const {
+        const float a = at(x);
+        if (a < end) {
+            const float b = a + MAGIC, r = a - (b - MAGIC);
+            const uint32_t n = MASS ? __float_as_uint(fmaf(fmaf(r, 8.0f, -1024.0f), r, MAGIC + 65536.0f)) & 0x7FFFFFu : 1u;
+            atomicAdd(bins + (__float_as_uint(b) & 0x7FFFFFu), n);
+        }
+    }
+    // A value that is above all x of the bins from `bin` on, or, `under`, below all x of the bins up to it: next to the bin's end, by more than `at` is off.
+    __device__ float end_of(uint32_t bin, bool under) const {
+        if (under && bin >= SM_BINS - 1) return -3.402823466e38f;
+        if (!under && bin == 0) return INFINITY;
+        const float x = m - ((float)bin + (under ? 0.5f : -0.5f)) / scale, off = (fabsf(m) + fabsf(x)) * 0x1p-21f;
+        return under ? fmaxf(x - off, -3.402823466e38f) : x + off;
     }
 };
 
@@ -680,11 +695,36 @@ __device__ __forceinline__ void hand_over(Team& t, uint32_t Shared::*counter) {
     for (uint32_t i = threadIdx.x; i < min(n, SM_CANDIDATES) && s.place + i < SM_CANDIDATES; i += SM_THREADS) lead->list[s.place + i] = s.list[i];
 }
 
+struct Settings {
+    bool greedy;
+    double warm;            // temperature
+    uint32_t top_k;         // 0: all
+    float top_p, min_p, uniform;
+    __device__ Settings(const b200bpe_choice& how, uint32_t row, uint32_t vocab) {
+        const float t = how.temperature ? how.temperature[row] : 1.0f;
+        greedy = !how.uniform || !(t >= SM_GREEDY_BELOW);
+        warm = greedy ? 1.0 : fmin((double)t, 3.4e38);
+        top_k = greedy || !how.top_k ? 0u : how.top_k[row];
+        if (top_k >= vocab) top_k = 0u;
+        const float p = greedy || !how.top_p ? 1.0f : how.top_p[row], m = greedy || !how.min_p ? 0.0f : how.min_p[row];
+        top_p = p < 1.0f ? fmaxf(p, 0.0f) : 1.0f;
+        min_p = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
+        const float u = greedy ? 0.0f : how.uniform[row];
+        uniform = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
+    }
+    // The smallest x that min_p keeps.
+    __device__ uint32_t min_key(float m) const {
+        return min_p > 0.0f ? key_of(__double2float_ru((double)m + log((double)min_p) * warm)) : LOWEST_KEY;
+    }
+};
+
 // The part of the row's order at which a running sum, from the largest x on, reaches `target`: of weights (MASS) or of tokens.
 // s.bins are filled in all CTAs (weights: in parts of 2^16 of the bin's largest), and a barrier of the cluster is behind that.
-// Returns what is kept up to and with the token that reaches it, the same in every CTA.
+// Returns what is kept up to and with the token that reaches it, the same in every CTA.  With `set` (nothing was taken away before) `found` is where the
+// draw falls, if that is known by the way; the caller has its owner at 0xFFFFFFFF.
 template <bool MASS>
-__device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& bins, double target, double share, double margin) {
+__device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& bins, double target, double share, double margin, const Settings* set,
+                       uint32_t whole, Draw& found) {
     Shared& s = t.s;
     const int shift = (int)sl.lo - (int)sl.lead;
     // every CTA adds up a part of the bins for all
@@ -696,8 +736,9 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
         here[k] = 0;
         if (busy && k < per) {
             unsigned long long n = 0;
+#pragma unroll 8
             for (uint32_t c = 0; c < t.C; c++) n += t.peer(c)->bins[first + k];
-            here[k] = MASS ? (double)n * exp(-(double)(first + k) / 64) / 65536.0 : (double)n;
+            here[k] = MASS ? (double)((float)n * (__expf(-(float)(first + k) / 64) / 65536.0f)) : (double)n;
         }
         sum += here[k];
     }
@@ -707,8 +748,8 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     // (t.total's barriers: the parts of a bin may be read until here)
     double a = threadIdx.x == 0 ? all : 0.0, none = 0;
     t.total(a, none);
-    for (uint32_t c = 0; c < t.rank; c++) at += t.part(0, c);
-    const double slack = MASS ? 1.0 / 32768 : 0.0;          // 2^-17 a weight, 2 * 2^-24 * 2048 / 64 its place, and what the target is off
+    at += warp_sum(t.lane < t.rank ? t.part(0, t.lane) : 0.0);
+    const double slack = MASS ? 1.0 / 32768 : 0.0;          // 2^-17 a weight, 2 * 2^-24 * 2048 / 64 its place, the bins' weights, and what the target is off
 #pragma unroll
     for (uint32_t k = 0; k < SM_BINS / SM_THREADS; k++) {
         if (k >= per || !busy) break;
@@ -723,19 +764,19 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     }
     t.sync();
     // sums of what is above the border's bins; what lies in them goes to the first CTA
-    const uint32_t from = s.border[0], to = max(s.border[1], from);
+    const float high = bins.end_of(s.border[0], false), low = bins.end_of(max(s.border[0], s.border[1]), true);
     double above = 0, count = 0;
     each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
         const float v[4] = {x.x, x.y, x.z, x.w};
-        float part = 0;
         uint32_t in = 0;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint32_t b = bins.of(v[k]);
-            if (b < from) part += MASS ? w.quick(v[k]) : 1.0f;
-            else if (b <= to && v[k] > -INFINITY) in |= 1u << k;
+        for (int k = 0; k < 4; k++) in |= (uint32_t)(v[k] <= high && v[k] >= low) << k;
+        if (x.x > high || x.y > high || x.z > high || x.w > high) {
+            float e[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) e[k] = v[k] > high ? MASS ? w.quick(v[k]) : 1.0f : 0.0f;
+            above += (double)((e[0] + e[1]) + (e[2] + e[3]));
         }
-        above += (double)part;
         gather(t, &s.candidates, s.list, v, in, p + shift);      // (the list lies where the bins were)
     });
     hand_over(t, &Shared::candidates);
@@ -755,6 +796,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                 }
                 // neighbours to a thread; flag 1: a sum was near, 2: the bins were misjudged
                 double v[SM_EACH], mine = 0;
+#pragma unroll
                 for (uint32_t k = 0; k < SM_EACH; k++) {
                     const uint32_t i = threadIdx.x * SM_EACH + k;
                     v[k] = i < n ? (MASS ? w.exact(value_of((uint32_t)(s.list[i] >> 32))) : 1.0) : 0.0;
@@ -762,6 +804,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                 }
                 if (threadIdx.x == 0) { s.flag = 0u; s.place = n ? n - 1 : 0u; }
                 double ignored, sum = above + t.before(mine, &ignored);
+#pragma unroll
                 for (uint32_t k = 0; k < SM_EACH; k++) {
                     const double next = sum + v[k];
                     const uint32_t i = threadIdx.x * SM_EACH + k;
@@ -773,15 +816,45 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                 if (MASS && threadIdx.x == 0 && above >= target - near) s.flag = 1u + turn;
                 if (MASS && threadIdx.x == SM_THREADS - 1 && sum < target + near) s.flag = 1u + turn;
                 __syncthreads();
+                const unsigned long long e = s.list[s.place];
+                const Kept kept = n ? Kept{(uint32_t)(e >> 32), ~(uint32_t)e + 1u} : Kept{LOWEST_KEY, 0u};
+                const uint32_t near_some = s.flag;
+                Draw draw{0xFFFFFFFFu, 0.0, 0.0};
+                if (MASS && set && near_some == 0u && turn == 0 && set->min_key(w.m) <= kept.key) {
+                    // Nothing else takes tokens away: the kept ones' weights by CTA are known, and so is where the draw falls.
+                    __syncthreads();
+#pragma unroll
+                    for (uint32_t k = 0; k < SM_EACH; k++) {
+                        const uint32_t i = threadIdx.x * SM_EACH + k;
+                        if (i < size) s.list[i] = s.list[i] << 32 | __float_as_uint(i <= s.place ? (float)v[k] : 0.0f);
+                    }
+                    __syncthreads();
+                                        for (uint32_t c = t.warp; c < t.C; c += SM_WARPS) {
+                        double part = 0;
+                        for (uint32_t i = t.lane; i < n; i += 32) {
+                            const uint32_t token = ~(uint32_t)(s.list[i] >> 32);
+                            if (token - c * whole < whole) part += (double)__uint_as_float((uint32_t)s.list[i]);
+                        }
+                        part = warp_sum(part);
+                        if (t.lane == 0) s.step_mass[c] = part + t.part(0, c);
+                    }
+                    __syncthreads();
+                    const double part = t.lane < t.C ? s.step_mass[t.lane] : 0.0;
+                    draw.target = (double)set->uniform * warp_sum(part);
+                    draw.owner = t.first_above(part, 0.0, draw.target, &draw.base);
+                }
                 if (threadIdx.x < t.C) {
                     Shared* p = t.peer(threadIdx.x);
-                    const unsigned long long e = s.list[s.place];
-                    p->kept = n ? Kept{(uint32_t)(e >> 32), ~(uint32_t)e + 1u} : Kept{LOWEST_KEY, 0u};
-                    p->cut_at[0] = s.flag;
+                    p->kept = kept;
+                    p->draw = draw;
+                    p->again = near_some;
                 }
             }
             t.sync();
-            if (s.cut_at[0] == 0u) return s.kept;
+            if (s.again == 0u) {
+                found = s.draw;
+                return s.kept;
+            }
             if (turn == 1) break;
             // weights in 64 bits: of all, for the target, and of what is above
             double total = 0;
@@ -792,7 +865,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                     if (v[k] > -INFINITY) {
                         const double e = w.exact(v[k]);
                         total += e;
-                        if (bins.of(v[k]) < from) above += e;
+                        if (v[k] > high) above += e;
                     }
             });
             t.total(total, above);
@@ -817,54 +890,31 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
         t.total(mass, none);
         return mass;
     };
-    uint32_t low = LOWEST_KEY + 1u, high = key_of(w.m);      // from_key(low) reaches the target, as far as any does
-    while (low < high) {
-        const uint32_t mid = low + (high - low + 1u) / 2u;
-        if (from_key(mid) >= target) low = mid;
-        else high = mid - 1u;
+    uint32_t least = LOWEST_KEY + 1u, most = key_of(w.m);      // from_key(least) reaches the target, as far as any does
+    while (least < most) {
+        const uint32_t mid = least + (most - least + 1u) / 2u;
+        if (from_key(mid) >= target) least = mid;
+        else most = mid - 1u;
     }
-    const double more = from_key(low + 1u), each = MASS ? w.exact(value_of(low)) : 1.0;
+    const double more = from_key(least + 1u), each = MASS ? w.exact(value_of(least)) : 1.0;
     double ties = each > 0 ? fmax(ceil((target - more) / each), 1.0) : 1.0;
     if (ties > 1.0 && more + (ties - 1.0) * each >= target) ties -= 1.0;
     double equal = 0;
     each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
-        equal += (double)((key_of(x.x) == low) + (key_of(x.y) == low) + (key_of(x.z) == low) + (key_of(x.w) == low));
+        equal += (double)((key_of(x.x) == least) + (key_of(x.y) == least) + (key_of(x.z) == least) + (key_of(x.w) == least));
     });
     t.total(equal, none);
-    if (ties >= equal) return Kept{low, 0xFFFFFFFFu};
+    if (ties >= equal) return Kept{least, 0xFFFFFFFFu};
     double base;
     const uint32_t owner = t.first_above(t.lane < t.C ? t.part(0, t.lane) : 0.0, 0.0, ties - 0.5, &base);
     if (t.rank == owner) {
         bool near;
-        const uint32_t p = find_place(t, sl, base, ties - 0.5, 0.0, &near, [&](uint32_t, float x) { return key_of(x) == low ? 1.0 : 0.0; });
+        const uint32_t p = find_place(t, sl, base, ties - 0.5, 0.0, &near, [&](uint32_t, float x) { return key_of(x) == least ? 1.0 : 0.0; });
         if (threadIdx.x < t.C) t.peer(threadIdx.x)->cut_at[1] = p + shift + 1u;
     }
     t.sync();
-    return Kept{low, s.cut_at[1]};
+    return Kept{least, s.cut_at[1]};
 }
-
-struct Settings {
-    bool greedy;
-    double warm;            // temperature
-    uint32_t top_k;         // 0: all
-    float top_p, min_p, uniform;
-    __device__ Settings(const b200bpe_choice& how, uint32_t row, uint32_t vocab) {
-        const float t = how.temperature ? how.temperature[row] : 1.0f;
-        greedy = !how.uniform || !(t >= SM_GREEDY_BELOW);
-        warm = greedy ? 1.0 : fmin((double)t, 3.4e38);
-        top_k = greedy || !how.top_k ? 0u : how.top_k[row];
-        if (top_k >= vocab) top_k = 0u;
-        const float p = greedy || !how.top_p ? 1.0f : how.top_p[row], m = greedy || !how.min_p ? 0.0f : how.min_p[row];
-        top_p = p < 1.0f ? fmaxf(p, 0.0f) : 1.0f;
-        min_p = m > 0.0f ? fminf(m, 1.0f) : 0.0f;
-        const float u = greedy ? 0.0f : how.uniform[row];
-        uniform = u > 0.0f ? fminf(u, 1.0f) : 0.0f;
-    }
-    // The smallest x that min_p keeps.
-    __device__ uint32_t min_key(float m) const {
-        return min_p > 0.0f ? key_of(__double2float_ru((double)m + log((double)min_p) * warm)) : LOWEST_KEY;
-    }
-};
 
 // The choice among the candidates in the first CTA's list, which has all of the top_k largest: everything in 64 bits.  Called by that CTA's threads.
 __device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& set, uint32_t n, float* x) {
@@ -1047,6 +1097,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
 
     // The kept tokens.
     Kept kept{LOWEST_KEY, 0u};
+    Draw draw{0xFFFFFFFFu, 0.0, 0.0};
     if (quick_k) {
         // At least top_k x are not below the largest value that 2^l of the CTAs have 1/2^l of top_k for.
         float from = -INFINITY;
@@ -1062,13 +1113,14 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
             }
 #pragma unroll
             for (int o = 16; o; o >>= 1) from = fmaxf(from, __shfl_xor_sync(0xFFFFFFFFu, from, o));
+            from = fmaxf(from, -3.402823466e38f);        // (-infinity is never chosen)
         }
         Shared* lead = t.peer(0);
         each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
             const float v[4] = {x.x, x.y, x.z, x.w};
             uint32_t in = 0;
 #pragma unroll
-            for (int k = 0; k < 4; k++) in |= (uint32_t)(v[k] >= from && v[k] > -INFINITY) << k;
+            for (int k = 0; k < 4; k++) in |= (uint32_t)(v[k] >= from) << k;
             gather(t, &s.quick_candidates, s.list, v, in, p + shift);
         });
         hand_over(t, &Shared::quick_candidates);
@@ -1091,15 +1143,10 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         // (what weighs less than e^-32 does not matter to top_p; it may to top_k, where a temperature is low)
         const Bins bins(m, fmax(32.0 * set.warm, 24.0));
         each_four(sl, t.warp, [&](uint32_t, const float4& x) {
-            const float v[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint32_t b = bins.of(v[k]);
-                if (b < SM_BINS - 1) atomicAdd(&s.bins[b], 1u);
-            }
+            for (float v : {x.x, x.y, x.z, x.w}) bins.put<false>(s.bins, v, SM_BINS - 1.5f);
         });
         t.sync();
-        kept = border<false>(t, sl, w, bins, (double)set.top_k, -1.0, 0.0);
+        kept = border<false>(t, sl, w, bins, (double)set.top_k, -1.0, 0.0, nullptr, 0u, draw);
     }
     if (by_p) {
         double whole = all, none = 0;
@@ -1113,21 +1160,14 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         if (set.top_p > 0.0f) {
             const Bins bins(m, 32.0 * set.warm);
             // All that lie lower than this weigh less than half of what top_p leaves out.
-            float lowest = (float)(SM_BINS - 1);
-            if (set.top_p < 0.999f) lowest = fminf(lowest, 64.0f * logf((float)((double)vocab / (0.5 * (1.0 - set.top_p) * whole))) + 1.0f);
+            float end = SM_BINS - 1.5f;
+            if (set.top_p < 0.999f) end = fminf(end, 64.0f * logf((float)((double)vocab / (0.5 * (1.0 - set.top_p) * whole))) + 1.0f);
             each_four(sl, t.warp, [&](uint32_t, const float4& x) {
-                const float v[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float at = bins.at(v[k]);
-                    if (at < lowest) {
-                        const uint32_t b = Bins::whole(at);
-                        atomicAdd(&s.bins[b], Bins::weight(at, b));
-                    }
-                }
+                for (float v : {x.x, x.y, x.z, x.w}) bins.put<true>(s.bins, v, end);
             });
             t.sync();
-            k = border<true>(t, sl, w, bins, (double)set.top_p * whole, by_k ? -1.0 : (double)set.top_p, margin);
+            k = border<true>(t, sl, w, bins, (double)set.top_p * whole, by_k ? -1.0 : (double)set.top_p, margin, by_k ? nullptr : &set,
+                             slice_tokens(vocab, t.C), draw);
         } else {
             uint32_t token = 0xFFFFFFFFu;
             for (uint32_t c = 0; c < t.C; c++)
@@ -1140,32 +1180,46 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     if (min_key > kept.key) kept = {min_key, 0xFFFFFFFFu};
 
     // The draw.
-    auto chosen = [&](auto exact, bool known, uint32_t* place) {         // whether this CTA has the token
+    auto chosen = [&](auto exact, const Draw& draw, uint32_t* place) {         // whether this CTA has the token; every warp's sum is in s.warp_mass
         constexpr bool EXACT = decltype(exact)::value;
-        if (known) {
-            if (threadIdx.x < t.C) s.part_cta[0][t.par][threadIdx.x] = s.best[threadIdx.x].sum * Stats::power(s.best[threadIdx.x].n - n) * unit;
-            if (threadIdx.x < SM_WARPS) s.warp_mass[threadIdx.x] = s.part_warp[0][threadIdx.x] * Stats::power(s.n_warp[threadIdx.x] - n) * unit;
-            __syncthreads();
-        } else {
-            double mass = kept_mass<EXACT>(sl, t.warp, w, kept), none = 0;
-            t.total(mass, none);
-        }
-        const double here = t.lane < t.C ? t.part(0, t.lane) : 0.0, target = (double)set.uniform * warp_sum(here);
-        double base;
-        const uint32_t owner = t.first_above(here, 0.0, target, &base);
-        if (t.rank == owner) {
+        if (t.rank == draw.owner) {
             bool near;
-            *place = find_place(t, sl, base, target, EXACT ? 0.0 : margin, &near, [&](uint32_t p, float x) {
+            *place = find_place(t, sl, draw.base, draw.target, EXACT ? 0.0 : margin, &near, [&](uint32_t p, float x) {
                 return kept.has(x, p + shift) ? (EXACT ? w.exact(x) : (double)w.quick(x) * unit) : 0.0;
             });
             if (!EXACT && threadIdx.x < t.C) t.peer(threadIdx.x)->cut_at[0] = near;
         }
-        if (!EXACT) t.sync();
-        return t.rank == owner;
+        return t.rank == draw.owner;
     };
+    auto falls = [&](double part) {          // a lane's part: that of a CTA
+        Draw d;
+        d.target = (double)set.uniform * warp_sum(part);
+        d.owner = t.first_above(part, 0.0, d.target, &d.base);
+        return d;
+    };
+    if (draw.owner != 0xFFFFFFFFu) {
+        if (t.rank == draw.owner) {
+            const double mass = warp_sum(kept_mass<false>(sl, t.warp, w, kept));
+            if (t.lane == 0) s.warp_mass[t.warp] = mass;
+            __syncthreads();
+        }
+    } else if (!by_k && !by_p && set.min_p == 0.0f) {
+        draw = falls(t.lane < t.C ? s.best[t.lane].sum * Stats::power(s.best[t.lane].n - n) * unit : 0.0);
+        if (threadIdx.x < SM_WARPS) s.warp_mass[threadIdx.x] = s.part_warp[0][threadIdx.x] * Stats::power(s.n_warp[threadIdx.x] - n) * unit;
+        __syncthreads();
+    } else {
+        double mass = kept_mass<false>(sl, t.warp, w, kept), none = 0;
+        t.total(mass, none);
+        draw = falls(t.lane < t.C ? t.part(0, t.lane) : 0.0);
+    }
     uint32_t place = 0;
-    bool mine = chosen(std::false_type{}, !by_k && !by_p && set.min_p == 0.0f, &place);
-    if (s.cut_at[0]) mine = chosen(std::true_type{}, false, &place);
+    bool mine = chosen(std::false_type{}, draw, &place);
+    t.sync();
+    if (s.cut_at[0]) {
+        double mass = kept_mass<true>(sl, t.warp, w, kept), none = 0;
+        t.total(mass, none);
+        mine = chosen(std::true_type{}, falls(t.lane < t.C ? t.part(0, t.lane) : 0.0), &place);
+    }
     if (mine && threadIdx.x == 0) answer(place + shift, buf[place]);
 }
 
