@@ -10,7 +10,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from .token_sampler import IDS, device_of
+from .token_sampler import IDS, raw_stream, row_of, table_of
 
 
 class TokenGrammar:
@@ -25,7 +25,7 @@ class TokenGrammar:
             raise ValueError("transitions: 1 to 65,535 states")
         if ends.shape != (table.shape[0],):
             raise ValueError("accepting: one value a state")
-        entries = [bytes(e) for e in vocab]
+        entries = vocab if isinstance(vocab, list) and set(map(type, vocab)) == {bytes} else [bytes(e) for e in vocab]
         if not entries:
             raise ValueError("vocab: no entries")
         if endToken is not None and not 0 <= endToken < len(entries):
@@ -44,24 +44,27 @@ class TokenGrammar:
     def _ready(self):
         if self._h is None:
             raise RuntimeError("TokenGrammar is destroyed")
-        import torch
-        return torch.cuda.current_stream(self._engine.device_index).cuda_stream
+        return raw_stream(self._engine.device_index)
 
     def allowedTokens(self, states, out=None):
         """states [rows] → mask int32 [rows, (vocabSize + 31) // 32] (or `out`, at least as wide): the tokens with bytes, all of which the automaton
         takes from the row's state, and the end token in an accepting state.  A state that is none (-1) allows nothing."""
         stream, at = self._ready(), self._engine.device_index
-        address, rows, words = device_of(states, "states", at, IDS, (None,)), states.shape[0], (self.vocabSize + 31) // 32
+        address, words = row_of(states, "states", at, IDS, None), (self.vocabSize + 31) >> 5
+        rows = states.shape[0]
         if out is None:
             import torch
             out = states.new_empty((rows, words), dtype=torch.int32)
+            p_out = out.data_ptr()
         else:
-            device_of(out, "out", at, IDS, (rows, None))
+            p_out = table_of(out, "out", at, IDS, rows)
             if out.shape[1] < words:
                 raise ValueError(f"out: {out.shape[1]} words, the vocabulary needs {words}")
             if rows > 1 and out.stride(0) < words:
                 raise ValueError("out: rows overlap")
-        _lib.check(_lib.lib().b200bpe_grammar_mask(self._h, address, rows, out.data_ptr(), out.stride(0), stream), "b200bpe_grammar_mask")
+        status = _lib.lib().b200bpe_grammar_mask(self._h, address, rows, p_out, out.stride(0), stream)
+        if status:
+            _lib.check(status, "b200bpe_grammar_mask")
         return out
 
     def advance(self, states, tokens, history=None, lengths=None, out=None, lengthsOut=None):
@@ -71,33 +74,34 @@ class TokenGrammar:
         With history [rows, room] and lengths: tokens are also written behind each row's history, and → (states, new lengths) (or
         `lengthsOut`, which may be lengths).  No token, and a full row, changes neither."""
         stream, at = self._ready(), self._engine.device_index
-        rows = states.shape[0] if len(states.shape) else None
-        p_states, p_tokens = device_of(states, "states", at, IDS, (None,)), device_of(tokens, "tokens", at, IDS, (rows,))
+        p_states = row_of(states, "states", at, IDS, None)
+        rows = states.shape[0]
+        p_tokens = row_of(tokens, "tokens", at, IDS, rows)
         import torch
         if out is None:
             out = states.new_empty(rows, dtype=torch.int32)
-        p_out = device_of(out, "out", at, IDS, (rows,))
-        if history is None:
-            if lengths is not None or lengthsOut is not None:
-                raise ValueError("lengths: without a history")
-            _lib.check(_lib.lib().b200bpe_grammar_advance(self._h, p_states, p_tokens, rows, p_out, None, 0, 0, None, None, stream),
-                       "b200bpe_grammar_advance")
-            return out
-        if lengths is None:
-            raise ValueError("lengths: needed with a history")
-        p_lengths = device_of(lengths, "lengths", at, IDS, (rows,))
-        p_history = device_of(history, "history", at, IDS, (rows, None))
-        if rows > 1 and history.stride(0) < history.shape[1]:
-            raise ValueError("history: rows overlap")
-        if lengthsOut is None:
-            lengthsOut = lengths.new_empty(rows, dtype=torch.int32)
-        p_new = device_of(lengthsOut, "lengthsOut", at, IDS, (rows,))
-        room = history.shape[1]
-        if rows and not room:             # (an empty tensor has no address)
-            p_history = p_lengths
-        _lib.check(_lib.lib().b200bpe_grammar_advance(self._h, p_states, p_tokens, rows, p_out, p_history, history.stride(0), room, p_lengths, p_new,
-                                                      stream), "b200bpe_grammar_advance")
-        return out, lengthsOut
+        p_out = row_of(out, "out", at, IDS, rows)
+        p_history = p_lengths = p_new = None
+        stride = room = 0
+        if history is not None:
+            if lengths is None:
+                raise ValueError("lengths: needed with a history")
+            p_lengths = row_of(lengths, "lengths", at, IDS, rows)
+            p_history = table_of(history, "history", at, IDS, rows)
+            stride, room = history.stride(0), history.shape[1]
+            if rows > 1 and stride < room:
+                raise ValueError("history: rows overlap")
+            if lengthsOut is None:
+                lengthsOut = lengths.new_empty(rows, dtype=torch.int32)
+            p_new = row_of(lengthsOut, "lengthsOut", at, IDS, rows)
+            if rows and not room:             # (an empty tensor has no address)
+                p_history = p_lengths
+        elif lengths is not None or lengthsOut is not None:
+            raise ValueError("lengths: without a history")
+        status = _lib.lib().b200bpe_grammar_advance(self._h, p_states, p_tokens, rows, p_out, p_history, stride, room, p_lengths, p_new, stream)
+        if status:
+            _lib.check(status, "b200bpe_grammar_advance")
+        return out if history is None else (out, lengthsOut)
 
     def destroy(self):
         if self._h is not None:

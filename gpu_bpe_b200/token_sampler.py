@@ -10,94 +10,134 @@ import ctypes as C
 
 from . import _lib
 
-DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
-IDS, FLOATS = ("torch.int32", "torch.uint32"), ("torch.float32",)
+# Types by name; a dtype object joins its name when it is met first (its name takes as long to make as the rest of a check).
+LOGITS = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+IDS = {"torch.int32": 0, "torch.uint32": 0}
+FLOATS = {"torch.float32": 0}
+MAX_VOCAB, MAX_BIASES = 327680, 1024
 
 
-def device_of(t, name, index, kinds, shape):
-    """Refuses a tensor that is not of these types and this shape (None: any size), dense within its rows, on GPU `index`; its address."""
-    if str(getattr(t, "dtype", None)) not in kinds:
-        raise ValueError(f"{name}: a tensor of {' or '.join(kinds)} is needed")
+def _refuse(t, name, index, kinds, shape):
+    """What is wrong with a tensor that row_of or table_of did not take at sight; nothing, if it is its type's first."""
+    kind = getattr(t, "dtype", None)
+    if kind not in kinds:
+        if str(kind) not in kinds:
+            raise ValueError(f"{name}: a tensor of {' or '.join(k for k in kinds if isinstance(k, str))} is needed")
+        kinds[kind] = kinds[str(kind)]
     if len(t.shape) != len(shape) or any(want is not None and want != got for want, got in zip(shape, t.shape)):
         raise ValueError(f"{name}: shape {tuple(t.shape)} where {tuple(shape)} is needed")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}: elements of a row must lie next to one another")
-    if t.device.type != "cuda" or t.device.index != index:
+    if t.get_device() != index:
         raise ValueError(f"{name}: on {t.device}, the engine is on cuda:{index}")
+
+
+def row_of(t, name, index, kinds, rows):
+    """Address of a tensor [rows] (None: any number) of one of these types on GPU `index`."""
+    try:
+        if t.dtype in kinds and t.get_device() == index and len(t.shape) == 1 and (rows is None or t.shape[0] == rows) and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(t, name, index, kinds, (rows,))
     return t.data_ptr()
+
+
+def table_of(t, name, index, kinds, rows):
+    """The same of a tensor [rows, any number], its rows at any distance."""
+    try:
+        if t.dtype in kinds and t.get_device() == index and len(t.shape) == 2 and (rows is None or t.shape[0] == rows) and t.stride(1) == 1:
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(t, name, index, kinds, (rows, None))
+    return t.data_ptr()
+
+
+_stream_of = None
+
+
+def raw_stream(index):
+    """Torch's current stream on GPU `index`, as a number."""
+    global _stream_of
+    if _stream_of is None:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)       # (a tenth of a microsecond; the stream as an object takes two)
+        _stream_of = raw or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+    return _stream_of(index)
 
 
 class TokenSampler:
     def __init__(self, engine, vocabSize: int):
         self._engine, self.vocabSize = engine, int(vocabSize)
         self._h = None
-        if not 1 <= self.vocabSize <= 327680:
-            raise ValueError("vocabSize: 1 to 327,680 tokens")
+        if not 1 <= self.vocabSize <= MAX_VOCAB:
+            raise ValueError(f"vocabSize: 1 to {MAX_VOCAB:,} tokens")
         h = C.c_void_p()
         _lib.check(_lib.lib().b200bpe_sampler_create(engine.ctx, self.vocabSize, C.byref(h)), "b200bpe_sampler_create")
         self._h = h
 
-    def _row(self, value, name, rows, kinds, like):
-        """Address of one value a row; a plain number stands for all rows (the tensor that holds it is returned, too)."""
+    def _row(self, keep, value, name, rows, kinds, like):
+        """Address of one value a row; None has none, a plain number stands for all rows."""
+        if value is None:
+            return None
         if isinstance(value, (int, float)):
             import torch
             value = torch.full((rows,), value, dtype=torch.int32 if kinds is IDS else torch.float32, device=like.device)
-        return device_of(value, name, self._engine.device_index, kinds, (rows,)), value
+            keep.append(value)
+        return row_of(value, name, self._engine.device_index, kinds, rows)
 
     def _logits(self, keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows):
         if self._h is None:
             raise RuntimeError("TokenSampler is destroyed")
         at = self._engine.device_index
-        p = _lib.Logits()
-        p.struct_size = C.sizeof(_lib.Logits)
-        p.logits = device_of(logits, "logits", at, DTYPES, (None, None))
-        rows = logits.shape[0]
-        if logits.shape[1] < self.vocabSize:
-            raise ValueError(f"logits: {logits.shape[1]} columns, the vocabulary has {self.vocabSize} tokens")
-        p.dtype, p.n_rows, p.row_stride = DTYPES[str(logits.dtype)], rows, logits.stride(0)
+        p_logits = table_of(logits, "logits", at, LOGITS, None)
+        rows, columns = logits.shape
+        if columns < self.vocabSize:
+            raise ValueError(f"logits: {columns} columns, the vocabulary has {self.vocabSize} tokens")
+        p_history = p_lengths = p_prompt = p_rep = p_pres = p_freq = p_ids = p_biases = p_mask = p_which = None
+        history_stride = room = n_bias = bias_stride = mask_stride = mask_rows = 0
         if history is not None:
             if lengths is None:
                 raise ValueError("lengths: needed with a history")
-            p.history = device_of(history, "history", at, IDS, (rows, None))
-            p.history_stride, p.history_cap = history.stride(0), history.shape[1]
-            for field, value, name, kinds in (("lengths", lengths, "lengths", IDS), ("prompt_lengths", promptLengths, "promptLengths", IDS),
-                                              ("repetition", repetition, "repetition", FLOATS), ("presence", presence, "presence", FLOATS),
-                                              ("frequency", frequency, "frequency", FLOATS)):
-                if value is not None:
-                    address, tensor = self._row(value, name, rows, kinds, logits)
-                    setattr(p, field, address)
-                    keep.append(tensor)
-            if not history.shape[1]:
-                p.history = p.lengths = p.prompt_lengths = p.repetition = p.presence = p.frequency = None
-        elif any(x is not None for x in (lengths, promptLengths, repetition, presence, frequency)):
+            p_history = table_of(history, "history", at, IDS, rows)
+            history_stride, room = history.stride(0), history.shape[1]
+            p_lengths = self._row(keep, lengths, "lengths", rows, IDS, logits)
+            p_prompt = self._row(keep, promptLengths, "promptLengths", rows, IDS, logits)
+            p_rep = self._row(keep, repetition, "repetition", rows, FLOATS, logits)
+            p_pres = self._row(keep, presence, "presence", rows, FLOATS, logits)
+            p_freq = self._row(keep, frequency, "frequency", rows, FLOATS, logits)
+            if not room:
+                p_history = p_lengths = p_prompt = p_rep = p_pres = p_freq = None
+        elif not (lengths is None and promptLengths is None and repetition is None and presence is None and frequency is None):
             raise ValueError("history: needed for lengths and penalties")
-        if (biasTokens is None) != (biases is None):
-            raise ValueError("biasTokens and biases: one without the other")
-        if biasTokens is not None:
-            p.n_bias = biasTokens.shape[-1] if len(biasTokens.shape) == 2 else 0
-            if p.n_bias > 1024:
-                raise ValueError("biasTokens: at most 1,024 a row")
-            p.bias_tokens = device_of(biasTokens, "biasTokens", at, IDS, (rows, None))
-            p.biases = device_of(biases, "biases", at, FLOATS, (rows, p.n_bias))
-            p.bias_stride = biasTokens.stride(0)
-            if biases.stride(0) != biasTokens.stride(0) and rows > 1 and p.n_bias:
+        if biasTokens is not None or biases is not None:
+            if biasTokens is None or biases is None:
+                raise ValueError("biasTokens and biases: one without the other")
+            p_ids = table_of(biasTokens, "biasTokens", at, IDS, rows)
+            n_bias, bias_stride = biasTokens.shape[1], biasTokens.stride(0)
+            if n_bias > MAX_BIASES:
+                raise ValueError(f"biasTokens: at most {MAX_BIASES:,} a row")
+            p_biases = table_of(biases, "biases", at, FLOATS, rows)
+            if biases.shape[1] != n_bias:
+                raise ValueError(f"biases: shape {tuple(biases.shape)} where {(rows, n_bias)} is needed")
+            if biases.stride(0) != bias_stride and rows > 1 and n_bias:
                 raise ValueError("biases: another distance between rows than biasTokens")
         if mask is not None:
-            p.mask = device_of(mask, "mask", at, IDS, (None, None))
-            p.n_mask_rows, p.mask_stride = mask.shape[0], mask.stride(0)
-            if mask.shape[1] < (self.vocabSize + 31) // 32:
+            p_mask = table_of(mask, "mask", at, IDS, None)
+            mask_rows, mask_stride = mask.shape[0], mask.stride(0)
+            if mask.shape[1] < (self.vocabSize + 31) >> 5:
                 raise ValueError(f"mask: {mask.shape[1]} words, the vocabulary needs {(self.vocabSize + 31) // 32}")
             if maskRows is not None:
-                p.mask_rows = device_of(maskRows, "maskRows", at, IDS, (rows,))
-            elif mask.shape[0] != rows:
-                raise ValueError(f"mask: {mask.shape[0]} rows for {rows} rows of logits, and no maskRows")
+                p_which = row_of(maskRows, "maskRows", at, IDS, rows)
+                if rows and not mask_rows:
+                    raise ValueError("mask: no rows")
+            elif mask_rows != rows:
+                raise ValueError(f"mask: {mask_rows} rows for {rows} rows of logits, and no maskRows")
         elif maskRows is not None:
             raise ValueError("maskRows: needs a mask")
-        return p
-
-    def _stream(self):
-        import torch
-        return torch.cuda.current_stream(self._engine.device_index).cuda_stream
+        return _lib.Logits(LOGITS_BYTES, LOGITS[logits.dtype], rows, n_bias, p_logits, logits.stride(0), p_history, history_stride, p_lengths, p_prompt,
+                           room, mask_rows, p_rep, p_pres, p_freq, p_ids, p_biases, bias_stride, p_mask, mask_stride, p_which)
 
     def adjustLogits(self, logits, out=None, history=None, lengths=None, promptLengths=None, repetition=None, presence=None, frequency=None,
                      biasTokens=None, biases=None, mask=None, maskRows=None):
@@ -112,13 +152,16 @@ class TokenSampler:
         p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
         if out is None:
             out = logits.new_empty((logits.shape[0], self.vocabSize))
-        else:
-            device_of(out, "out", self._engine.device_index, (str(logits.dtype),), (logits.shape[0], None))
-            if out.shape[1] < self.vocabSize:
-                raise ValueError(f"out: {out.shape[1]} columns, the vocabulary has {self.vocabSize} tokens")
-            if out.shape[0] > 1 and out.stride(0) < self.vocabSize:
-                raise ValueError("out: rows overlap")
-        _lib.check(_lib.lib().b200bpe_sampler_adjust(self._h, C.byref(p), out.data_ptr(), out.stride(0), self._stream()), "b200bpe_sampler_adjust")
+        address = table_of(out, "out", self._engine.device_index, LOGITS, logits.shape[0])
+        if out.dtype != logits.dtype:
+            raise ValueError(f"out: a tensor of {logits.dtype} is needed")
+        if out.shape[1] < self.vocabSize:
+            raise ValueError(f"out: {out.shape[1]} columns, the vocabulary has {self.vocabSize} tokens")
+        if out.stride(0) < self.vocabSize and out.shape[0] > 1:
+            raise ValueError("out: rows overlap")
+        status = _lib.lib().b200bpe_sampler_adjust(self._h, C.byref(p), address, out.stride(0), raw_stream(self._engine.device_index))
+        if status:
+            _lib.check(status, "b200bpe_sampler_adjust")
         return out
 
     def sample(self, logits, uniform=None, temperature=None, topK=None, topP=None, minP=None, history=None, lengths=None, promptLengths=None,
@@ -133,26 +176,27 @@ class TokenSampler:
         keep = []
         p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
         rows = logits.shape[0]
-        c = _lib.Choice()
-        c.struct_size = C.sizeof(_lib.Choice)
-        if uniform is None:
-            if any(x is not None for x in (temperature, topK, topP, minP)):
-                raise ValueError("uniform: needed to draw")
-        else:
-            c.uniform = device_of(uniform, "uniform", self._engine.device_index, FLOATS, (rows,))
-            for field, value, name, kinds in (("temperature", temperature, "temperature", FLOATS), ("top_k", topK, "topK", IDS),
-                                              ("top_p", topP, "topP", FLOATS), ("min_p", minP, "minP", FLOATS)):
-                if value is not None:
-                    address, tensor = self._row(value, name, rows, kinds, logits)
-                    setattr(c, field, address)
-                    keep.append(tensor)
+        p_uniform = p_warm = p_k = p_p = p_m = None
+        if uniform is not None:
+            p_uniform = row_of(uniform, "uniform", self._engine.device_index, FLOATS, rows)
+            p_warm = self._row(keep, temperature, "temperature", rows, FLOATS, logits)
+            p_k = self._row(keep, topK, "topK", rows, IDS, logits)
+            p_p = self._row(keep, topP, "topP", rows, FLOATS, logits)
+            p_m = self._row(keep, minP, "minP", rows, FLOATS, logits)
+        elif not (temperature is None and topK is None and topP is None and minP is None):
+            raise ValueError("uniform: needed to draw")
         import torch
         tokens, logprobs = logits.new_empty(rows, dtype=torch.int32), logits.new_empty(rows, dtype=torch.float32)
-        c.tokens_out, c.logprobs_out = tokens.data_ptr(), logprobs.data_ptr()
-        _lib.check(_lib.lib().b200bpe_sampler_sample(self._h, C.byref(p), C.byref(c), self._stream()), "b200bpe_sampler_sample")
+        c = _lib.Choice(CHOICE_BYTES, 0, p_uniform, p_warm, p_k, p_p, p_m, tokens.data_ptr(), logprobs.data_ptr())
+        status = _lib.lib().b200bpe_sampler_sample(self._h, C.byref(p), C.byref(c), raw_stream(self._engine.device_index))
+        if status:
+            _lib.check(status, "b200bpe_sampler_sample")
         return tokens, logprobs
 
     def destroy(self):
         if self._h is not None:
             _lib.lib().b200bpe_sampler_destroy(self._h)
             self._h = None
+
+
+LOGITS_BYTES, CHOICE_BYTES = C.sizeof(_lib.Logits), C.sizeof(_lib.Choice)

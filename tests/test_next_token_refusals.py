@@ -21,6 +21,12 @@ class Fake:
     def stride(self, i=None):
         return self._strides if i is None else self._strides[i]
 
+    def is_contiguous(self):
+        return len(self.shape) == 1 and self._strides == (1,)
+
+    def get_device(self):
+        return self.device.index if self.device.type == "cuda" else -1
+
     def data_ptr(self):
         return 4096
 
