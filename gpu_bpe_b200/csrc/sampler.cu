@@ -117,26 +117,31 @@ struct Span {
 // Which places of a slice are not plain logits: bit p & 31 of word p >> 5 is place p's.
 template <uint32_t MOST>
 struct Special {
-    uint32_t deny[MOST / 32 + 1];        // masked
-    uint32_t seen[MOST / 32 + 1];        // in the history: the buffer has its x
+    uint32_t any[MOST / 32 + 1];         // masked, or in the history
+    uint32_t seen[MOST / 32 + 1];        // in the history: the buffer has its x (-infinity if it is masked)
     uint32_t todo[MOST / 32 + 1];        // not yet, it has its marks
 };
 
 // Makes `special`, and x of the places in the history: there, penalties cost a scattered load a token, not a test and a division for every lane of
 // the row.  Returns whether there are any special places.  Called by all threads of the CTA; ends with a barrier.
-// Each CTA reads the whole history of its row, and counts what is its own: a history is short beside a row, and L2 has it.
+// Each CTA reads the whole history of its row, and counts what is its own: a history is short beside a row, and L2 has it.  What a thread reads first
+// does not depend on anything else that is read, so that a row's settings and the first of its history are one wait.
 template <uint32_t MOST, class T>
-__device__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const T* row, const Slice& s, const MaskRow& mask, Special<MOST>& special) {
+__device__ __forceinline__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const T* row, const Slice& s, const MaskRow& mask, Special<MOST>& special) {
+    constexpr int EACH = 8;                          // of a history, a thread keeps at hand
     Penalty pen{1.0f, 0.0f, 0.0f};
-    uint32_t n_seen = 0, prompt = 0;
+    uint32_t n_seen = 0, prompt = 0, t[EACH];
+    const uint32_t* h = nullptr;
     if (in.history) {
+        h = in.history + (uint64_t)s.row * in.history_stride;
+        n_seen = min(in.lengths[s.row], in.history_cap);
+        if (in.prompt_lengths) prompt = in.prompt_lengths[s.row];
         if (in.repetition) pen.repetition = in.repetition[s.row];
         if (in.presence) pen.presence = in.presence[s.row];
         if (in.frequency) pen.frequency = in.frequency[s.row];
-        if (pen.repetition != 1.0f || pen.presence != 0.0f || pen.frequency != 0.0f) {
-            n_seen = min(in.lengths[s.row], in.history_cap);
-            prompt = in.prompt_lengths ? in.prompt_lengths[s.row] : 0u;
-        }
+#pragma unroll
+        for (int k = 0; k < EACH; k++) t[k] = threadIdx.x + k * SM_THREADS < in.history_cap ? h[threadIdx.x + k * SM_THREADS] : 0u;
+        if (pen.repetition == 1.0f && pen.presence == 0.0f && pen.frequency == 0.0f) n_seen = 0;
     }
     if (n_seen == 0 && !mask.words && !mask.none) return false;
     const uint32_t words = (s.padded + 31u) / 32u, mask_words = (vocab + 31u) / 32u;
@@ -147,7 +152,7 @@ __device__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const T* 
             const uint32_t lo = w >= 0 && w < (int)mask_words ? mask.words[w] : 0u, hi = w + 1 < (int)mask_words ? mask.words[w + 1] : 0u;
             allowed = __funnelshift_r(lo, hi, (uint32_t)v & 31u);
         }
-        special.deny[i] = ~allowed;
+        special.any[i] = ~allowed;
         special.seen[i] = special.todo[i] = 0u;
     }
     uint32_t* marks = reinterpret_cast<uint32_t*>(s.buf);
@@ -155,39 +160,42 @@ __device__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const T* 
         for (uint32_t i = threadIdx.x * 4; i < s.padded; i += SM_THREADS * 4) *reinterpret_cast<uint4*>(marks + i) = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     if (n_seen) {
-        const uint32_t* h = in.history + (uint64_t)s.row * in.history_stride;
-        // counted; then the first to come back to a place makes its x
-        for (int turn = 0; turn < 2; turn++) {
-            for (uint32_t i0 = threadIdx.x; i0 < n_seen; i0 += SM_THREADS * 4) {
-                uint32_t t[4];
+        auto count = [&](uint32_t p, bool in_prompt) {           // whether this is the first at its place
+            if ((in_prompt ? atomicOr(&marks[p], Penalty::SEEN) : atomicAdd(&marks[p], 1u)) != 0u) return false;
+            atomicOr(&special.any[p >> 5], 1u << (p & 31u));
+            atomicOr(&special.seen[p >> 5], 1u << (p & 31u));
+            return true;
+        };
+        auto make = [&](uint32_t v, uint32_t p, T x) { s.buf[p] = mask.allows(v) ? pen.on(as_float(x), marks[p]) : -INFINITY; };
+        if (n_seen <= EACH * SM_THREADS) {
+            // counted; when all are, the first at a place makes its x
+            T x[EACH];
+            uint32_t firsts = 0;
 #pragma unroll
-                for (int k = 0; k < 4; k++) t[k] = i0 + k * SM_THREADS < n_seen ? h[i0 + k * SM_THREADS] - s.lo : 0xFFFFFFFFu;
-                if (turn == 0) {
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if (t[k] >= s.len) continue;
-                        const uint32_t p = t[k] + s.lead;
-                        const uint32_t had = i0 + k * SM_THREADS < prompt ? atomicOr(&marks[p], Penalty::SEEN) : atomicAdd(&marks[p], 1u);
-                        if (had == 0u) {
-                            atomicOr(&special.seen[p >> 5], 1u << (p & 31u));
-                            atomicOr(&special.todo[p >> 5], 1u << (p & 31u));
-                        }
-                    }
-                } else {
-                    T x[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if (t[k] < s.len && !(atomicAnd(&special.todo[(t[k] + s.lead) >> 5], ~(1u << ((t[k] + s.lead) & 31u))) >> ((t[k] + s.lead) & 31u) & 1u))
-                            t[k] = 0xFFFFFFFFu;
-                        if (t[k] < s.len) x[k] = row[t[k]];
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        if (t[k] < s.len) s.buf[t[k] + s.lead] = pen.on(as_float(x[k]), marks[t[k] + s.lead]);
+            for (int k = 0; k < EACH; k++) {
+                const uint32_t i = threadIdx.x + k * SM_THREADS, at = t[k] - s.lo;
+                if (i < n_seen && at < s.len && count(at + s.lead, i < prompt)) {
+                    firsts |= 1u << k;
+                    x[k] = row[at];
                 }
             }
             __syncthreads();
+#pragma unroll
+            for (int k = 0; k < EACH; k++)
+                if (firsts >> k & 1u) make(t[k], t[k] - s.lo + s.lead, x[k]);
+        } else {
+            // the same, but who was the first is not remembered: the first to come back to a place makes its x
+            for (uint32_t i = threadIdx.x; i < n_seen; i += SM_THREADS) {
+                const uint32_t at = h[i] - s.lo, p = at + s.lead;
+                if (at < s.len && count(p, i < prompt)) atomicOr(&special.todo[p >> 5], 1u << (p & 31u));
+            }
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < n_seen; i += SM_THREADS) {
+                const uint32_t v = h[i], at = v - s.lo, p = at + s.lead, bit = 1u << (p & 31u);
+                if (at < s.len && (special.todo[p >> 5] & bit) && (atomicAnd(&special.todo[p >> 5], ~bit) & bit)) make(v, p, row[at]);
+            }
         }
+        __syncthreads();
     }
     return true;
 }
@@ -222,18 +230,19 @@ __device__ __forceinline__ void each_adjusted(const T* row, const Slice& s, uint
             for (uint32_t k = 0; k < N; k++) v[k] = now.get(k);
             if (any_special) {
                 constexpr uint32_t ALL = (1u << N) - 1u;
-                const uint32_t deny = special.deny[p >> 5] >> (p & 31u) & ALL, seen = special.seen[p >> 5] >> (p & 31u) & ALL;
-                if (seen) {
+                if (const uint32_t any = special.any[p >> 5] >> (p & 31u) & ALL) {
+                    const uint32_t seen = special.seen[p >> 5] >> (p & 31u);
+                    if (seen & ALL) {
 #pragma unroll
-                    for (uint32_t k = 0; k < N; k += 4) {
-                        const float4 x = *reinterpret_cast<const float4*>(s.buf + p + k);
-                        v[k] = seen >> k & 1u ? x.x : v[k];
-                        v[k + 1] = seen >> (k + 1) & 1u ? x.y : v[k + 1];
-                        v[k + 2] = seen >> (k + 2) & 1u ? x.z : v[k + 2];
-                        v[k + 3] = seen >> (k + 3) & 1u ? x.w : v[k + 3];
+                        for (uint32_t k = 0; k < N; k += 4) {
+                            const float4 x = *reinterpret_cast<const float4*>(s.buf + p + k);
+                            v[k] = seen >> k & 1u ? x.x : v[k];
+                            v[k + 1] = seen >> (k + 1) & 1u ? x.y : v[k + 1];
+                            v[k + 2] = seen >> (k + 2) & 1u ? x.z : v[k + 2];
+                            v[k + 3] = seen >> (k + 3) & 1u ? x.w : v[k + 3];
+                        }
                     }
-                }
-                if (deny) {
+                    const uint32_t deny = any & ~seen;
 #pragma unroll
                     for (uint32_t k = 0; k < N; k++) v[k] = deny >> k & 1u ? -INFINITY : v[k];
                 }
@@ -408,9 +417,9 @@ constexpr uint32_t SM_QUICK_K = 512;             // top_k up to which a row's ca
 
 // Which token is chosen depends on sums of weights: on the first running sum that is above a border.  Sums are made of weights in 32 bits,
 // w = 2^(x c - n) with c = log2 e / temperature, and added in 64 bits.  Against the exact weights, up to a factor that all have in common, the
-// exponent is off by the roundings of c and of the product's difference, together 2 * 2^-24 (m - x) c + 2^-24, the exponential by 2^-22 of itself, and up to
+// exponent is off by the roundings of log2 e, c and the product's difference, together 2.5 * 2^-24 (m - x) c + 2^-24, the exponential by 2^-22 of itself, and up to
 // eight weights are added in 32 bits first, three roundings: a sum is off by at most
-//     E = sum w * 2^-24 * (10 + 2 ln 2 (m - x) c),
+//     E = sum w * 2^-24 * (10 + 2.5 ln 2 (m - x) c),
 // with two for the factor that brings such sums to the unit of the others, where that matters.
 // The mean of (m - x) c under the weights is their entropy less log2 Z, Z = sum w / max w, so at most log2(tokens / Z).  A border that is a share u of
 // the sum S has its part of the same errors: a running sum s is off from u S by (1 - u) times what s is off less u times what the rest is off, less than
@@ -622,17 +631,57 @@ __device__ uint32_t find_place(Team& t, const Slice& sl, double base, double tar
     return s.place;
 }
 
-// Descending order of n numbers (n a power of two, at most SM_CANDIDATES).
-__device__ void sort_down(unsigned long long* a, uint32_t n) {
-    for (uint32_t size = 2; size <= n; size <<= 1)
-        for (uint32_t step = size >> 1; step; step >>= 1) {
-            for (uint32_t i = threadIdx.x; i < n / 2; i += SM_THREADS) {
-                const uint32_t lo = (i & ~(step - 1u)) << 1 | (i & (step - 1u)), hi = lo + step;
-                const unsigned long long x = a[lo], y = a[hi];
-                if ((x < y) == ((lo & size) == 0)) { a[lo] = y; a[hi] = x; }
-            }
+// Descending order of E * SM_THREADS numbers, E to a thread (its neighbours in the order): a bitonic network, whose steps run within a thread, by
+// shuffles, and between warps through `list`, which has them in the end.
+template <int E>
+__device__ __forceinline__ void sort_threads(unsigned long long* list) {
+    constexpr uint32_t N = E * SM_THREADS;
+    const uint32_t i0 = threadIdx.x * E;
+    unsigned long long a[E];
+#pragma unroll
+    for (int k = 0; k < E; k++) a[k] = list[i0 + k];
+    auto keep = [](unsigned long long mine, unsigned long long other, bool larger) { return (mine > other) == larger ? mine : other; };
+#pragma unroll 1
+    for (uint32_t size = 2; size <= N; size <<= 1) {
+#pragma unroll 1
+        for (uint32_t step = size >> 1; step >= 32 * E; step >>= 1) {
             __syncthreads();
+#pragma unroll
+            for (int k = 0; k < E; k++) list[i0 + k] = a[k];
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < E; k++) a[k] = keep(a[k], list[(i0 + k) ^ step], ((i0 & step) == 0) == ((i0 & size) == 0));
         }
+#pragma unroll 1
+        for (uint32_t step = min(size >> 1, 16u * E); step >= E; step >>= 1)
+#pragma unroll
+            for (int k = 0; k < E; k++) a[k] = keep(a[k], __shfl_xor_sync(0xFFFFFFFFu, a[k], step / E), ((i0 & step) == 0) == ((i0 & size) == 0));
+#pragma unroll
+        for (int step = E / 2; step >= 1; step >>= 1)
+            if (size > (uint32_t)step)
+#pragma unroll
+                for (int k = 0; k < E; k++)
+                    if ((k & step) == 0) {
+                        const bool down = ((i0 + k) & size) == 0;
+                        const unsigned long long x = a[k], y = a[k + step];
+                        if ((x < y) == down) { a[k] = y; a[k + step] = x; }
+                    }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < E; k++) list[i0 + k] = a[k];
+    __syncthreads();
+}
+// Of n numbers (zeros behind them are added); returns how many lie at a thread: thread i has those from i * that on.
+__device__ __forceinline__ uint32_t sort_down(unsigned long long* list, uint32_t n) {
+    const uint32_t size = n <= SM_THREADS ? SM_THREADS : n <= 2 * SM_THREADS ? 2 * SM_THREADS : 4 * SM_THREADS;
+    static_assert(SM_CANDIDATES == 4 * SM_THREADS, "the list's room");
+    for (uint32_t i = n + threadIdx.x; i < size; i += SM_THREADS) list[i] = 0ull;
+    __syncthreads();
+    if (size == SM_THREADS) sort_threads<1>(list);
+    else if (size == 2 * SM_THREADS) sort_threads<2>(list);
+    else sort_threads<4>(list);
+    return size / SM_THREADS;
 }
 
 // Bins of x, from the largest downwards: SM_BINS of them over `range`, each round its middle; the last one takes the rest.
@@ -784,22 +833,17 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     t.total(above, count);
     const uint32_t n = t.peer(0)->candidates;
     if (n <= SM_CANDIDATES) {
+        uint32_t each = 1;
         for (int turn = 0; turn < 2; turn++) {
             // turn 1: again with the sums in 64 bits
             if (t.rank == 0) {
-                uint32_t size = 2;
-                while (size < n) size *= 2;
-                if (turn == 0) {
-                    for (uint32_t i = n + threadIdx.x; i < size; i += SM_THREADS) s.list[i] = 0ull;
-                    __syncthreads();
-                    sort_down(s.list, size);
-                }
+                if (turn == 0) each = sort_down(s.list, n);
                 // neighbours to a thread; flag 1: a sum was near, 2: the bins were misjudged
                 double v[SM_EACH], mine = 0;
 #pragma unroll
                 for (uint32_t k = 0; k < SM_EACH; k++) {
-                    const uint32_t i = threadIdx.x * SM_EACH + k;
-                    v[k] = i < n ? (MASS ? w.exact(value_of((uint32_t)(s.list[i] >> 32))) : 1.0) : 0.0;
+                    const uint32_t i = threadIdx.x * each + k;
+                    v[k] = k < each && i < n ? (MASS ? w.exact(value_of((uint32_t)(s.list[i] >> 32))) : 1.0) : 0.0;
                     mine += v[k];
                 }
                 if (threadIdx.x == 0) { s.flag = 0u; s.place = n ? n - 1 : 0u; }
@@ -807,7 +851,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
 #pragma unroll
                 for (uint32_t k = 0; k < SM_EACH; k++) {
                     const double next = sum + v[k];
-                    const uint32_t i = threadIdx.x * SM_EACH + k;
+                    const uint32_t i = k < each ? threadIdx.x * each + k : n;
                     if (i < n && sum < target && next >= target) s.place = i;
                     if (MASS && turn == 0 && i < n && (fabs(sum - target) <= margin || fabs(next - target) <= margin)) s.flag = 1u;
                     sum = next;
@@ -825,8 +869,8 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                     __syncthreads();
 #pragma unroll
                     for (uint32_t k = 0; k < SM_EACH; k++) {
-                        const uint32_t i = threadIdx.x * SM_EACH + k;
-                        if (i < size) s.list[i] = s.list[i] << 32 | __float_as_uint(i <= s.place ? (float)v[k] : 0.0f);
+                        const uint32_t i = threadIdx.x * each + k;
+                        if (k < each) s.list[i] = s.list[i] << 32 | __float_as_uint(i <= s.place ? (float)v[k] : 0.0f);
                     }
                     __syncthreads();
                                         for (uint32_t c = t.warp; c < t.C; c += SM_WARPS) {
@@ -919,14 +963,11 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
 // The choice among the candidates in the first CTA's list, which has all of the top_k largest: everything in 64 bits.  Called by that CTA's threads.
 __device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& set, uint32_t n, float* x) {
     Shared& s = t.s;
-    uint32_t size = 2;
-    while (size < n) size *= 2;
-    for (uint32_t i = n + threadIdx.x; i < size; i += SM_THREADS) s.list[i] = 0ull;
-    __syncthreads();
-    sort_down(s.list, size);
+    uint32_t each = sort_down(s.list, n);
     n = min(n, set.top_k);
     // neighbours to a thread
-    const uint32_t each = max(size / SM_THREADS, 1u), i0 = threadIdx.x * each, min_key = set.min_key(w.m);
+    uint32_t i0 = threadIdx.x * each;
+    const uint32_t min_key = set.min_key(w.m);
     double v[SM_EACH], mine = 0, all;
 #pragma unroll
     for (uint32_t k = 0; k < SM_EACH; k++) {
@@ -948,16 +989,15 @@ __device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& 
     __syncthreads();
 #pragma unroll
     for (uint32_t k = 0; k < SM_EACH; k++)
-        if (k < each && i0 + k < size) s.list[i0 + k] = e[k];
+        if (k < each) s.list[i0 + k] = e[k];
     __syncthreads();
-    size = 2;
-    while (size < n) size *= 2;              // (the first n, in the order of x, were looked at)
-    sort_down(s.list, size);
+    each = sort_down(s.list, n);             // (the first n, in the order of x, were looked at)
+    i0 = threadIdx.x * each;
     mine = 0;
     uint32_t filled = 0;
 #pragma unroll
     for (uint32_t k = 0; k < SM_EACH; k++) {
-        const unsigned long long c = k < each && i0 + k < size ? s.list[i0 + k] : 0ull;
+        const unsigned long long c = k < each ? s.list[i0 + k] : 0ull;
         v[k] = c ? w.exact(value_of((uint32_t)c)) : 0.0;
         if (v[k] > 0) filled = i0 + k;
         mine += v[k];
@@ -993,7 +1033,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     const Settings set(how, sl.row, vocab);
     const bool by_k = set.top_k != 0u, by_p = set.top_p < 1.0f, quick_k = by_k && set.top_k <= SM_QUICK_K;
     Stats stats;
-    stats.c = (float)(1.4426950408889634 / set.warm);
+    stats.c = __fdiv_rn(1.44269504f, (float)set.warm);
     {
         const MaskRow mask = mask_row(in, sl.row);
         const bool any_special = find_special(in, vocab, row, sl, mask, s.special);
@@ -1093,7 +1133,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         return;
     }
     all *= unit;
-    const double margin = all * (double)((10.0f + 1.4f * (log2f((float)vocab / (float)all) + 1.0f)) / 16777216.0f);
+    const double margin = all * (double)((10.0f + 1.75f * (log2f((float)vocab / (float)all) + 1.0f)) / 16777216.0f);
 
     // The kept tokens.
     Kept kept{LOWEST_KEY, 0u};
@@ -1118,6 +1158,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         Shared* lead = t.peer(0);
         each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
             const float v[4] = {x.x, x.y, x.z, x.w};
+            if (!__any_sync(0xFFFFFFFFu, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= from)) return;
             uint32_t in = 0;
 #pragma unroll
             for (int k = 0; k < 4; k++) in |= (uint32_t)(v[k] >= from) << k;
