@@ -421,9 +421,10 @@ constexpr uint32_t SM_QUICK_K = 512;             // top_k up to which a row's ca
 // eight weights are added in 32 bits first, three roundings: a sum is off by at most
 //     E = sum w * 2^-24 * (10 + 2.5 ln 2 (m - x) c),
 // with two for the factor that brings such sums to the unit of the others, where that matters.
-// The mean of (m - x) c under the weights is their entropy less log2 Z, Z = sum w / max w, so at most log2(tokens / Z).  A border that is a share u of
-// the sum S has its part of the same errors: a running sum s is off from u S by (1 - u) times what s is off less u times what the rest is off, less than
-// E.  Where a running sum that decides lies within E of the border, the row's sums are made again of weights in 64 bits.
+// The mean of (m - x) c under some tokens' weights is their entropy less log2 r, r = sum w / the row's largest w, so at most log2(tokens / r).  A border
+// that is a share u of a sum S has its part of the same errors: a running sum next to it is off from it by (1 - u) times what it is off itself, E(u S), less
+// u times what the rest is off, E((1 - u) S).  Where a running sum that decides lies within that of the border, the row's sums are made again of
+// weights in 64 bits.
 struct Weights {
     float m, c, n;              // the largest x, log2 e / temperature, the exponent that all quick weights are relative to
     double steps;               // 64 log2 e / temperature
@@ -442,6 +443,13 @@ struct Weights {
     __device__ __forceinline__ double to_largest() const { return (double)exp2f((float)power_of_largest()); }        // quick's unit in exact's
 };
 
+// How far a running sum may be off from a share of the sum, both of quick weights; or, `exact`, from a border that is exact.
+__device__ __forceinline__ double how_near(uint32_t vocab, double sum, double share, bool exact) {
+    auto off = [&](float r) { return r > 0.0f ? r * (10.0f + 1.75f * (1.0f + log2f((float)vocab / r))) : 0.0f; };
+    const float a = off((float)(share * sum)), b = off((float)((1.0 - share) * sum));
+    return (double)(exact ? a : (float)(1.0 - share) * a + (float)share * b) * (1.01 / 16777216.0);
+}
+
 // What of the row is kept: x with a larger key, and those with the key in front of token `end`.
 struct Kept {
     uint32_t key, end;
@@ -451,8 +459,8 @@ struct Kept {
     }
 };
 
-// Where a draw falls: in which CTA's slice, what is in front of that, and the sum to be passed.
-struct Draw { uint32_t owner; double base, target; };      // (owner 0xFFFFFFFF: not known)
+// Where a draw falls: in which CTA's slice, what is in front of that, the sum to be passed, and what is near that.
+struct Draw { uint32_t owner; double base, target, near; };      // (owner 0xFFFFFFFF: not known)
 struct Best { float m, n; uint32_t at, pad; double sum; float cut[4]; };       // a CTA's part of what the first exchange brings
 
 struct Shared {
@@ -773,7 +781,8 @@ struct Settings {
 // draw falls, if that is known by the way; the caller has its owner at 0xFFFFFFFF.
 template <bool MASS>
 __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& bins, double target, double share, double margin, const Settings* set,
-                       uint32_t whole, Draw& found) {
+                       uint32_t vocab, Draw& found) {
+    const uint32_t whole = slice_tokens(vocab, t.C);
     Shared& s = t.s;
     const int shift = (int)sl.lo - (int)sl.lead;
     // every CTA adds up a part of the bins for all
@@ -863,7 +872,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                 const unsigned long long e = s.list[s.place];
                 const Kept kept = n ? Kept{(uint32_t)(e >> 32), ~(uint32_t)e + 1u} : Kept{LOWEST_KEY, 0u};
                 const uint32_t near_some = s.flag;
-                Draw draw{0xFFFFFFFFu, 0.0, 0.0};
+                Draw draw{0xFFFFFFFFu, 0.0, 0.0, 0.0};
                 if (MASS && set && near_some == 0u && turn == 0 && set->min_key(w.m) <= kept.key) {
                     // Nothing else takes tokens away: the kept ones' weights by CTA are known, and so is where the draw falls.
                     __syncthreads();
@@ -884,7 +893,9 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                     }
                     __syncthreads();
                     const double part = t.lane < t.C ? s.step_mass[t.lane] : 0.0;
-                    draw.target = (double)set->uniform * warp_sum(part);
+                    const double stay = warp_sum(part);
+                    draw.target = (double)set->uniform * stay;
+                    draw.near = how_near(vocab, stay, set->uniform, false);
                     draw.owner = t.first_above(part, 0.0, draw.target, &draw.base);
                 }
                 if (threadIdx.x < t.C) {
@@ -1076,15 +1087,25 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         if (quick_k && t.warp < 4) {
             // cut[l]: at least top_k / 2^l of this slice are not below it.  The largest keys by their upper half that so many threads' largest x have.
             const uint32_t wanted = (set.top_k + (1u << t.warp) - 1u) >> t.warp;
-            uint32_t k[SM_THREADS / 32], cut = 0u;
+            uint32_t k[SM_THREADS / 32], most = 0u, least = 0xFFFFu;
 #pragma unroll
-            for (int i = 0; i < SM_THREADS / 32; i++) k[i] = s.keys[i * 32 + t.lane] >> 16;
-            for (uint32_t bit = 0x8000u; bit; bit >>= 1) {
+            for (int i = 0; i < SM_THREADS / 32; i++) {
+                k[i] = s.keys[i * 32 + t.lane] >> 16;
+                most = max(most, k[i]);
+                least = min(least, k[i]);
+            }
+            most = __reduce_max_sync(0xFFFFFFFFu, most);
+            least = __reduce_min_sync(0xFFFFFFFFu, least);
+            // (the bits that all of them have alike need no looking at, if there are enough of them)
+            const uint32_t unlike = most == least ? 0u : 31u - __clz(most ^ least);
+            uint32_t cut = wanted <= SM_THREADS ? most & ~((2u << unlike) - 1u) : 0u;
+            for (uint32_t bit = most == least ? 0u : 1u << unlike; bit; bit >>= 1) {
                 uint32_t so_many = 0;
 #pragma unroll
                 for (int i = 0; i < SM_THREADS / 32; i++) so_many += k[i] >= (cut | bit);
                 if (__reduce_add_sync(0xFFFFFFFFu, so_many) >= wanted) cut |= bit;
             }
+            if (most == least && wanted <= SM_THREADS) cut = most;
             if (t.lane == 0 && cut > LOWEST_KEY >> 16) s.cut[t.warp] = value_of(cut << 16);
         }
         __syncthreads();
@@ -1114,6 +1135,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         }
         return;
     }
+    if (set.greedy && (t.rank != 0 || t.warp != 0)) return;
     const Weights w{m, stats.c, n, 64 * 1.4426950408889634 / set.warm, s.table};
     const double unit = w.to_largest();
     all = warp_sum(t.lane < t.C ? s.best[t.lane].sum * Stats::power(s.best[t.lane].n - n) : 0.0);
@@ -1133,11 +1155,10 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         return;
     }
     all *= unit;
-    const double margin = all * (double)((10.0f + 1.75f * (log2f((float)vocab / (float)all) + 1.0f)) / 16777216.0f);
 
     // The kept tokens.
     Kept kept{LOWEST_KEY, 0u};
-    Draw draw{0xFFFFFFFFu, 0.0, 0.0};
+    Draw draw{0xFFFFFFFFu, 0.0, 0.0, 0.0};
     if (quick_k) {
         // At least top_k x are not below the largest value that 2^l of the CTAs have 1/2^l of top_k for.
         float from = -INFINITY;
@@ -1187,7 +1208,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
             for (float v : {x.x, x.y, x.z, x.w}) bins.put<false>(s.bins, v, SM_BINS - 1.5f);
         });
         t.sync();
-        kept = border<false>(t, sl, w, bins, (double)set.top_k, -1.0, 0.0, nullptr, 0u, draw);
+        kept = border<false>(t, sl, w, bins, (double)set.top_k, -1.0, 0.0, nullptr, vocab, draw);
     }
     if (by_p) {
         double whole = all, none = 0;
@@ -1207,8 +1228,8 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
                 for (float v : {x.x, x.y, x.z, x.w}) bins.put<true>(s.bins, v, end);
             });
             t.sync();
-            k = border<true>(t, sl, w, bins, (double)set.top_p * whole, by_k ? -1.0 : (double)set.top_p, margin, by_k ? nullptr : &set,
-                             slice_tokens(vocab, t.C), draw);
+            k = border<true>(t, sl, w, bins, (double)set.top_p * whole, by_k ? -1.0 : (double)set.top_p, how_near(vocab, whole, set.top_p, by_k),
+                             by_k ? nullptr : &set, vocab, draw);
         } else {
             uint32_t token = 0xFFFFFFFFu;
             for (uint32_t c = 0; c < t.C; c++)
@@ -1225,7 +1246,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         constexpr bool EXACT = decltype(exact)::value;
         if (t.rank == draw.owner) {
             bool near;
-            *place = find_place(t, sl, draw.base, draw.target, EXACT ? 0.0 : margin, &near, [&](uint32_t p, float x) {
+            *place = find_place(t, sl, draw.base, draw.target, EXACT ? 0.0 : draw.near, &near, [&](uint32_t p, float x) {
                 return kept.has(x, p + shift) ? (EXACT ? w.exact(x) : (double)w.quick(x) * unit) : 0.0;
             });
             if (!EXACT && threadIdx.x < t.C) t.peer(threadIdx.x)->cut_at[0] = near;
@@ -1234,7 +1255,9 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     };
     auto falls = [&](double part) {          // a lane's part: that of a CTA
         Draw d;
-        d.target = (double)set.uniform * warp_sum(part);
+        const double stay = warp_sum(part);
+        d.target = (double)set.uniform * stay;
+        d.near = how_near(vocab, stay, set.uniform, false);
         d.owner = t.first_above(part, 0.0, d.target, &d.base);
         return d;
     };

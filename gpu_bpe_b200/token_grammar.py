@@ -51,15 +51,15 @@ class TokenGrammar:
         takes from the row's state, and the end token in an accepting state.  A state that is none (-1) allows nothing."""
         stream, at = self._ready(), self._engine.device_index
         address, words = row_of(states, "states", at, IDS, None), (self.vocabSize + 31) >> 5
-        rows = states.shape[0]
+        rows = states.size(0)
         if out is None:
             import torch
             out = states.new_empty((rows, words), dtype=torch.int32)
             p_out = out.data_ptr()
         else:
             p_out = table_of(out, "out", at, IDS, rows)
-            if out.shape[1] < words:
-                raise ValueError(f"out: {out.shape[1]} words, the vocabulary needs {words}")
+            if out.size(1) < words:
+                raise ValueError(f"out: {out.size(1)} words, the vocabulary needs {words}")
             if rows > 1 and out.stride(0) < words:
                 raise ValueError("out: rows overlap")
         status = _lib.lib().b200bpe_grammar_mask(self._h, address, rows, p_out, out.stride(0), stream)
@@ -75,7 +75,7 @@ class TokenGrammar:
         `lengthsOut`, which may be lengths).  No token, and a full row, changes neither."""
         stream, at = self._ready(), self._engine.device_index
         p_states = row_of(states, "states", at, IDS, None)
-        rows = states.shape[0]
+        rows = states.size(0)
         p_tokens = row_of(tokens, "tokens", at, IDS, rows)
         import torch
         if out is None:
@@ -88,7 +88,7 @@ class TokenGrammar:
                 raise ValueError("lengths: needed with a history")
             p_lengths = row_of(lengths, "lengths", at, IDS, rows)
             p_history = table_of(history, "history", at, IDS, rows)
-            stride, room = history.stride(0), history.shape[1]
+            stride, room = history.stride(0), history.size(1)
             if rows > 1 and stride < room:
                 raise ValueError("history: rows overlap")
             if lengthsOut is None:

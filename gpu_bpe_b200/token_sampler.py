@@ -35,7 +35,7 @@ def _refuse(t, name, index, kinds, shape):
 def row_of(t, name, index, kinds, rows):
     """Address of a tensor [rows] (None: any number) of one of these types on GPU `index`."""
     try:
-        if t.dtype in kinds and t.get_device() == index and len(t.shape) == 1 and (rows is None or t.shape[0] == rows) and t.is_contiguous():
+        if t.dtype in kinds and t.get_device() == index and t.ndim == 1 and (rows is None or t.size(0) == rows) and t.is_contiguous():
             return t.data_ptr()
     except AttributeError:
         pass
@@ -46,7 +46,7 @@ def row_of(t, name, index, kinds, rows):
 def table_of(t, name, index, kinds, rows):
     """The same of a tensor [rows, any number], its rows at any distance."""
     try:
-        if t.dtype in kinds and t.get_device() == index and len(t.shape) == 2 and (rows is None or t.shape[0] == rows) and t.stride(1) == 1:
+        if t.dtype in kinds and t.get_device() == index and t.ndim == 2 and (rows is None or t.size(0) == rows) and t.stride(1) == 1:
             return t.data_ptr()
     except AttributeError:
         pass
@@ -92,7 +92,7 @@ class TokenSampler:
             raise RuntimeError("TokenSampler is destroyed")
         at = self._engine.device_index
         p_logits = table_of(logits, "logits", at, LOGITS, None)
-        rows, columns = logits.shape
+        rows, columns = logits.size(0), logits.size(1)
         if columns < self.vocabSize:
             raise ValueError(f"logits: {columns} columns, the vocabulary has {self.vocabSize} tokens")
         p_history = p_lengths = p_prompt = p_rep = p_pres = p_freq = p_ids = p_biases = p_mask = p_which = None
@@ -101,7 +101,7 @@ class TokenSampler:
             if lengths is None:
                 raise ValueError("lengths: needed with a history")
             p_history = table_of(history, "history", at, IDS, rows)
-            history_stride, room = history.stride(0), history.shape[1]
+            history_stride, room = history.stride(0), history.size(1)
             p_lengths = self._row(keep, lengths, "lengths", rows, IDS, logits)
             p_prompt = self._row(keep, promptLengths, "promptLengths", rows, IDS, logits)
             p_rep = self._row(keep, repetition, "repetition", rows, FLOATS, logits)
@@ -115,18 +115,18 @@ class TokenSampler:
             if biasTokens is None or biases is None:
                 raise ValueError("biasTokens and biases: one without the other")
             p_ids = table_of(biasTokens, "biasTokens", at, IDS, rows)
-            n_bias, bias_stride = biasTokens.shape[1], biasTokens.stride(0)
+            n_bias, bias_stride = biasTokens.size(1), biasTokens.stride(0)
             if n_bias > MAX_BIASES:
                 raise ValueError(f"biasTokens: at most {MAX_BIASES:,} a row")
             p_biases = table_of(biases, "biases", at, FLOATS, rows)
-            if biases.shape[1] != n_bias:
+            if biases.size(1) != n_bias:
                 raise ValueError(f"biases: shape {tuple(biases.shape)} where {(rows, n_bias)} is needed")
             if biases.stride(0) != bias_stride and rows > 1 and n_bias:
                 raise ValueError("biases: another distance between rows than biasTokens")
         if mask is not None:
             p_mask = table_of(mask, "mask", at, IDS, None)
-            mask_rows, mask_stride = mask.shape[0], mask.stride(0)
-            if mask.shape[1] < (self.vocabSize + 31) >> 5:
+            mask_rows, mask_stride = mask.size(0), mask.stride(0)
+            if mask.size(1) < (self.vocabSize + 31) >> 5:
                 raise ValueError(f"mask: {mask.shape[1]} words, the vocabulary needs {(self.vocabSize + 31) // 32}")
             if maskRows is not None:
                 p_which = row_of(maskRows, "maskRows", at, IDS, rows)
@@ -151,13 +151,13 @@ class TokenSampler:
         keep = []
         p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
         if out is None:
-            out = logits.new_empty((logits.shape[0], self.vocabSize))
-        address = table_of(out, "out", self._engine.device_index, LOGITS, logits.shape[0])
+            out = logits.new_empty((logits.size(0), self.vocabSize))
+        address = table_of(out, "out", self._engine.device_index, LOGITS, logits.size(0))
         if out.dtype != logits.dtype:
             raise ValueError(f"out: a tensor of {logits.dtype} is needed")
-        if out.shape[1] < self.vocabSize:
-            raise ValueError(f"out: {out.shape[1]} columns, the vocabulary has {self.vocabSize} tokens")
-        if out.stride(0) < self.vocabSize and out.shape[0] > 1:
+        if out.size(1) < self.vocabSize:
+            raise ValueError(f"out: {out.size(1)} columns, the vocabulary has {self.vocabSize} tokens")
+        if out.stride(0) < self.vocabSize and out.size(0) > 1:
             raise ValueError("out: rows overlap")
         status = _lib.lib().b200bpe_sampler_adjust(self._h, C.byref(p), address, out.stride(0), raw_stream(self._engine.device_index))
         if status:
@@ -175,7 +175,7 @@ class TokenSampler:
         where the largest is taken).  A row without an allowed token gives -1 and -inf; a NaN is never chosen."""
         keep = []
         p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
-        rows = logits.shape[0]
+        rows = logits.size(0)
         p_uniform = p_warm = p_k = p_p = p_m = None
         if uniform is not None:
             p_uniform = row_of(uniform, "uniform", self._engine.device_index, FLOATS, rows)

@@ -21,6 +21,13 @@ class Fake:
     def stride(self, i=None):
         return self._strides if i is None else self._strides[i]
 
+    @property
+    def ndim(self):
+        return len(self.shape)
+
+    def size(self, i):
+        return self.shape[i]
+
     def is_contiguous(self):
         return len(self.shape) == 1 and self._strides == (1,)
 
