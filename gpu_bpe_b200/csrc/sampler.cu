@@ -414,6 +414,7 @@ constexpr uint32_t LOWEST_KEY = 0x007FFFFFu;     // of -infinity
 constexpr uint32_t SM_BINS = 2048;
 constexpr uint32_t SM_CANDIDATES = 1024, SM_EACH = SM_CANDIDATES / SM_THREADS;
 constexpr uint32_t SM_QUICK_K = 512;             // top_k up to which a row's candidates are looked for without bins
+constexpr uint32_t SM_QUICK_P0 = 64, SM_QUICK_P1 = 256;    // where so few weigh what top_p keeps, they are looked for the same way
 
 // Which token is chosen depends on sums of weights: on the first running sum that is above a border.  Sums are made of weights in 32 bits,
 // w = 2^(x c - n) with c = log2 e / temperature, and added in 64 bits.  Against the exact weights, up to a factor that all have in common, the
@@ -971,11 +972,12 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     return Kept{least, s.cut_at[1]};
 }
 
-// The choice among the candidates in the first CTA's list, which has all of the top_k largest: everything in 64 bits.  Called by that CTA's threads.
-__device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& set, uint32_t n, float* x) {
+// The choice among the candidates in the first CTA's list, which are the row's largest: everything in 64 bits.  With whole < 0 the list has all of the
+// top_k; else top_p is a share of `whole`, known up to `near`, and the answer is whether the list has what it keeps.  Called by that CTA's threads.
+__device__ bool choose_from_list(Team& t, const Weights& w, const Settings& set, uint32_t n, double whole, double near, float* x, uint32_t* token) {
     Shared& s = t.s;
     uint32_t each = sort_down(s.list, n);
-    n = min(n, set.top_k);
+    if (set.top_k) n = min(n, set.top_k);
     // neighbours to a thread
     uint32_t i0 = threadIdx.x * each;
     const uint32_t min_key = set.min_key(w.m);
@@ -985,9 +987,10 @@ __device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& 
         v[k] = k < each && i0 + k < n ? w.exact(value_of((uint32_t)(s.list[i0 + k] >> 32))) : 0.0;
         mine += v[k];
     }
-    if (threadIdx.x == 0) s.place = 0u;
+    if (threadIdx.x == 0) { s.place = 0u; s.flag = 0u; }
     double sum = t.before(mine, &all);
-    const double enough = (double)set.top_p * all;
+    const double enough = (double)set.top_p * (whole < 0 ? all : whole);
+    bool open = whole >= 0 && all < enough + near;
     // what stays, with the token in front, so that the order becomes the tokens'
     unsigned long long e[SM_EACH];
 #pragma unroll
@@ -995,9 +998,12 @@ __device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& 
         const unsigned long long c = k < each && i0 + k < n ? s.list[i0 + k] : 0ull;
         const bool stays = c && (set.top_p >= 1.0f || sum < enough || i0 + k == 0u) && (uint32_t)(c >> 32) >= min_key;
         e[k] = stays ? c << 32 | c >> 32 : 0ull;
+        open |= whole >= 0 && c && (fabs(sum - enough) <= near || fabs(sum + v[k] - enough) <= near);
         sum += v[k];
     }
+    if (open) s.flag = 1u;
     __syncthreads();
+    if (s.flag) return false;
 #pragma unroll
     for (uint32_t k = 0; k < SM_EACH; k++)
         if (k < each) s.list[i0 + k] = e[k];
@@ -1025,7 +1031,8 @@ __device__ uint32_t choose_from_list(Team& t, const Weights& w, const Settings& 
     __syncthreads();
     const unsigned long long c = s.list[s.place];
     *x = value_of((uint32_t)c);
-    return ~(uint32_t)(c >> 32);
+    *token = ~(uint32_t)(c >> 32);
+    return true;
 }
 
 template <class T>
@@ -1043,6 +1050,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     first_loads(row, sl, ahead);
     const Settings set(how, sl.row, vocab);
     const bool by_k = set.top_k != 0u, by_p = set.top_p < 1.0f, quick_k = by_k && set.top_k <= SM_QUICK_K;
+    const bool quick_p = !by_k && by_p && set.top_p > 0.0f;
     Stats stats;
     stats.c = __fdiv_rn(1.44269504f, (float)set.warm);
     {
@@ -1073,8 +1081,8 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         if (threadIdx.x == 0) { s.at = 0xFFFFFFFFu; s.quick_candidates = 0u; }
         if (threadIdx.x < 4) s.cut[threadIdx.x] = -INFINITY;
         if (threadIdx.x < 64 && !set.greedy) s.table[threadIdx.x] = exp2((double)threadIdx.x / 64);
-        if (quick_k) s.keys[threadIdx.x] = key_of(stats.m);
-        else if (by_k || by_p)
+        if (quick_k || quick_p) s.keys[threadIdx.x] = key_of(stats.m);
+        else if (by_k)
             for (uint32_t i = threadIdx.x; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0u;
         __syncthreads();
         m = value_of(__reduce_max_sync(0xFFFFFFFFu, key_of(s.m_warp[t.lane % SM_WARPS])));
@@ -1084,9 +1092,10 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
             while (buf[p] != m) p++;
             atomicMin(&s.at, p + shift);
         }
-        if (quick_k && t.warp < 4) {
+        if (t.warp < (quick_k ? 4 : quick_p ? 2 : 0)) {
             // cut[l]: at least top_k / 2^l of this slice are not below it.  The largest keys by their upper half that so many threads' largest x have.
-            const uint32_t wanted = (set.top_k + (1u << t.warp) - 1u) >> t.warp;
+            // For top_p: as many as are this CTA's part of 64 and of 256, and in cut[2 + l] what they weigh (not less).
+            const uint32_t wanted = quick_k ? (set.top_k + (1u << t.warp) - 1u) >> t.warp : ((t.warp ? SM_QUICK_P1 : SM_QUICK_P0) + t.C - 1u) / t.C;
             uint32_t k[SM_THREADS / 32], most = 0u, least = 0xFFFFu;
 #pragma unroll
             for (int i = 0; i < SM_THREADS / 32; i++) {
@@ -1107,6 +1116,13 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
             }
             if (most == least && wanted <= SM_THREADS) cut = most;
             if (t.lane == 0 && cut > LOWEST_KEY >> 16) s.cut[t.warp] = value_of(cut << 16);
+            if (quick_p) {
+                double weight = 0;
+#pragma unroll
+                for (int i = 0; i < SM_THREADS / 32; i++) weight += k[i] >= cut ? (double)Stats::two_to(fmaf(value_of(k[i] << 16), stats.c, -n)) : 0.0;
+                weight = warp_sum(weight);
+                if (t.lane == 0) s.cut[2 + t.warp] = (float)weight;
+            }
         }
         __syncthreads();
         if (!again) cluster.barrier_wait();
@@ -1159,23 +1175,31 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     // The kept tokens.
     Kept kept{LOWEST_KEY, 0u};
     Draw draw{0xFFFFFFFFu, 0.0, 0.0, 0.0};
+    // Values that all of the top_k, or all that top_p keeps, are not below.
+    float from = -INFINITY;
+    bool quick = quick_k;
     if (quick_k) {
         // At least top_k x are not below the largest value that 2^l of the CTAs have 1/2^l of top_k for.
-        float from = -INFINITY;
-        {
-            for (uint32_t i = t.lane; i < 4 * SM_MAX_CLUSTER; i += 32) {
-                const uint32_t l = i / SM_MAX_CLUSTER, c = i % SM_MAX_CLUSTER;
-                if (c < t.C && 1u << l <= t.C) {
-                    const float mine = s.best[c].cut[l];
-                    uint32_t so_many = 0;
-                    for (uint32_t o = 0; o < t.C; o++) so_many += s.best[o].cut[l] >= mine;
-                    if (so_many >= 1u << l) from = fmaxf(from, mine);
-                }
+        for (uint32_t i = t.lane; i < 4 * SM_MAX_CLUSTER; i += 32) {
+            const uint32_t l = i / SM_MAX_CLUSTER, c = i % SM_MAX_CLUSTER;
+            if (c < t.C && 1u << l <= t.C) {
+                const float mine = s.best[c].cut[l];
+                uint32_t so_many = 0;
+                for (uint32_t o = 0; o < t.C; o++) so_many += s.best[o].cut[l] >= mine;
+                if (so_many >= 1u << l) from = fmaxf(from, mine);
             }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) from = fmaxf(from, __shfl_xor_sync(0xFFFFFFFFu, from, o));
-            from = fmaxf(from, -3.402823466e38f);        // (-infinity is never chosen)
         }
+        from = value_of(__reduce_max_sync(0xFFFFFFFFu, key_of(from)));
+    } else if (quick_p) {
+        // What the CTAs' parts of 64, or of 256, weigh is enough.
+        for (int l = 0; l < 2 && !quick; l++) {
+            const double weight = warp_sum(t.lane < t.C ? (double)s.best[t.lane].cut[2 + l] * Stats::power(s.best[t.lane].n - n) : 0.0) * unit;
+            quick = weight >= (double)set.top_p * all;
+            from = value_of(__reduce_min_sync(0xFFFFFFFFu, t.lane < t.C ? key_of(s.best[t.lane].cut[l]) : 0xFFFFFFFFu));
+        }
+    }
+    if (quick) {
+        from = fmaxf(from, -3.402823466e38f);            // (-infinity is never chosen)
         Shared* lead = t.peer(0);
         each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
             const float v[4] = {x.x, x.y, x.z, x.w};
@@ -1188,16 +1212,29 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         hand_over(t, &Shared::quick_candidates);
         t.sync();
         const uint32_t so_many = lead->quick_candidates;
-        cluster.barrier_arrive();
-        if (so_many <= SM_CANDIDATES) {
-            if (t.rank != 0) return;
-            float x;
-            const uint32_t token = choose_from_list(t, w, set, so_many, &x);
-            if (threadIdx.x == 0) answer(token, x);
-            cluster.barrier_wait();          // (the others have looked at the number)
-            return;
+        float x;
+        uint32_t token;
+        if (quick_k) {
+            cluster.barrier_arrive();
+            if (so_many <= SM_CANDIDATES) {
+                if (t.rank != 0) return;
+                choose_from_list(t, w, set, so_many, -1.0, 0.0, &x, &token);
+                if (threadIdx.x == 0) answer(token, x);
+                cluster.barrier_wait();          // (the others have looked at the number)
+                return;
+            }
+            cluster.barrier_wait();
+        } else if (so_many <= SM_CANDIDATES) {
+            if (t.rank == 0) {
+                const bool done = choose_from_list(t, w, set, so_many, all, how_near(vocab, all, set.top_p, false), &x, &token);
+                if (threadIdx.x == 0 && done) answer(token, x);
+                if (threadIdx.x < t.C) t.peer(threadIdx.x)->again = !done;
+            }
+            t.sync();
+            if (s.again == 0u) return;
         }
-        cluster.barrier_wait();
+    }
+    if (quick_k || quick_p) {
         for (uint32_t i = threadIdx.x; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0u;
         __syncthreads();
     }

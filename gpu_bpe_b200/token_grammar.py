@@ -50,19 +50,20 @@ class TokenGrammar:
         """states [rows] → mask int32 [rows, (vocabSize + 31) // 32] (or `out`, at least as wide): the tokens with bytes, all of which the automaton
         takes from the row's state, and the end token in an accepting state.  A state that is none (-1) allows nothing."""
         stream, at = self._ready(), self._engine.device_index
-        address, words = row_of(states, "states", at, IDS, None), (self.vocabSize + 31) >> 5
-        rows = states.size(0)
+        shape, words = states.shape[:1], (self.vocabSize + 31) >> 5
+        address = row_of(states, "states", at, IDS, shape)
+        rows = shape[0]
         if out is None:
             import torch
             out = states.new_empty((rows, words), dtype=torch.int32)
-            p_out = out.data_ptr()
+            p_out, stride = out.data_ptr(), words
         else:
-            p_out = table_of(out, "out", at, IDS, rows)
-            if out.size(1) < words:
-                raise ValueError(f"out: {out.size(1)} words, the vocabulary needs {words}")
-            if rows > 1 and out.stride(0) < words:
+            p_out, stride, columns = table_of(out, "out", at, IDS, rows)
+            if columns < words:
+                raise ValueError(f"out: {columns} words, the vocabulary needs {words}")
+            if rows > 1 and stride < words:
                 raise ValueError("out: rows overlap")
-        status = _lib.lib().b200bpe_grammar_mask(self._h, address, rows, p_out, out.stride(0), stream)
+        status = _lib.lib().b200bpe_grammar_mask(self._h, address, rows, p_out, stride, stream)
         if status:
             _lib.check(status, "b200bpe_grammar_mask")
         return out
@@ -74,26 +75,30 @@ class TokenGrammar:
         With history [rows, room] and lengths: tokens are also written behind each row's history, and → (states, new lengths) (or
         `lengthsOut`, which may be lengths).  No token, and a full row, changes neither."""
         stream, at = self._ready(), self._engine.device_index
-        p_states = row_of(states, "states", at, IDS, None)
-        rows = states.size(0)
-        p_tokens = row_of(tokens, "tokens", at, IDS, rows)
-        import torch
+        shape = states.shape[:1]
+        rows = shape[0] if shape else 0
+        p_states, p_tokens = row_of(states, "states", at, IDS, shape), row_of(tokens, "tokens", at, IDS, shape)
         if out is None:
-            out = states.new_empty(rows, dtype=torch.int32)
-        p_out = row_of(out, "out", at, IDS, rows)
+            import torch
+            out = states.new_empty(shape, dtype=torch.int32)
+            p_out = out.data_ptr()
+        else:
+            p_out = row_of(out, "out", at, IDS, shape)
         p_history = p_lengths = p_new = None
         stride = room = 0
         if history is not None:
             if lengths is None:
                 raise ValueError("lengths: needed with a history")
-            p_lengths = row_of(lengths, "lengths", at, IDS, rows)
-            p_history = table_of(history, "history", at, IDS, rows)
-            stride, room = history.stride(0), history.size(1)
+            p_lengths = row_of(lengths, "lengths", at, IDS, shape)
+            p_history, stride, room = table_of(history, "history", at, IDS, rows)
             if rows > 1 and stride < room:
                 raise ValueError("history: rows overlap")
             if lengthsOut is None:
-                lengthsOut = lengths.new_empty(rows, dtype=torch.int32)
-            p_new = row_of(lengthsOut, "lengthsOut", at, IDS, rows)
+                import torch
+                lengthsOut = lengths.new_empty(shape, dtype=torch.int32)
+                p_new = lengthsOut.data_ptr()
+            else:
+                p_new = row_of(lengthsOut, "lengthsOut", at, IDS, shape)
             if rows and not room:             # (an empty tensor has no address)
                 p_history = p_lengths
         elif lengths is not None or lengthsOut is not None:

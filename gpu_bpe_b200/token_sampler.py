@@ -32,26 +32,28 @@ def _refuse(t, name, index, kinds, shape):
         raise ValueError(f"{name}: on {t.device}, the engine is on cuda:{index}")
 
 
-def row_of(t, name, index, kinds, rows):
-    """Address of a tensor [rows] (None: any number) of one of these types on GPU `index`."""
+def row_of(t, name, index, kinds, shape):
+    """Address of a dense tensor of this shape, (rows,), of one of these types on GPU `index`."""
     try:
-        if t.dtype in kinds and t.get_device() == index and t.ndim == 1 and (rows is None or t.size(0) == rows) and t.is_contiguous():
+        if t.dtype in kinds and t.shape == shape and t.get_device() == index and t.is_contiguous():
             return t.data_ptr()
     except AttributeError:
         pass
-    _refuse(t, name, index, kinds, (rows,))
+    _refuse(t, name, index, kinds, shape)
     return t.data_ptr()
 
 
 def table_of(t, name, index, kinds, rows):
-    """The same of a tensor [rows, any number], its rows at any distance."""
+    """Address, distance between rows, and columns of a tensor [rows (None: any number), any number]; its rows may be at any distance."""
     try:
-        if t.dtype in kinds and t.get_device() == index and t.ndim == 2 and (rows is None or t.size(0) == rows) and t.stride(1) == 1:
-            return t.data_ptr()
+        if t.dtype in kinds and t.get_device() == index:
+            shape, strides = t.shape, t.stride()
+            if len(shape) == 2 and strides[1] == 1 and (rows is None or shape[0] == rows):
+                return t.data_ptr(), strides[0], shape[1]
     except AttributeError:
         pass
     _refuse(t, name, index, kinds, (rows, None))
-    return t.data_ptr()
+    return t.data_ptr(), t.stride(0), t.shape[1]
 
 
 _stream_of = None
@@ -77,22 +79,24 @@ class TokenSampler:
         _lib.check(_lib.lib().b200bpe_sampler_create(engine.ctx, self.vocabSize, C.byref(h)), "b200bpe_sampler_create")
         self._h = h
 
-    def _row(self, keep, value, name, rows, kinds, like):
+    def _row(self, keep, value, name, shape, kinds):
         """Address of one value a row; None has none, a plain number stands for all rows."""
         if value is None:
             return None
+        index = self._engine.device_index
         if isinstance(value, (int, float)):
             import torch
-            value = torch.full((rows,), value, dtype=torch.int32 if kinds is IDS else torch.float32, device=like.device)
+            value = torch.full(shape, value, dtype=torch.int32 if kinds is IDS else torch.float32, device=f"cuda:{index}")
             keep.append(value)
-        return row_of(value, name, self._engine.device_index, kinds, rows)
+        return row_of(value, name, index, kinds, shape)
 
     def _logits(self, keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows):
         if self._h is None:
             raise RuntimeError("TokenSampler is destroyed")
         at = self._engine.device_index
-        p_logits = table_of(logits, "logits", at, LOGITS, None)
-        rows, columns = logits.size(0), logits.size(1)
+        p_logits, row_stride, columns = table_of(logits, "logits", at, LOGITS, None)
+        shape = logits.shape[:1]
+        rows = shape[0]
         if columns < self.vocabSize:
             raise ValueError(f"logits: {columns} columns, the vocabulary has {self.vocabSize} tokens")
         p_history = p_lengths = p_prompt = p_rep = p_pres = p_freq = p_ids = p_biases = p_mask = p_which = None
@@ -100,13 +104,12 @@ class TokenSampler:
         if history is not None:
             if lengths is None:
                 raise ValueError("lengths: needed with a history")
-            p_history = table_of(history, "history", at, IDS, rows)
-            history_stride, room = history.stride(0), history.size(1)
-            p_lengths = self._row(keep, lengths, "lengths", rows, IDS, logits)
-            p_prompt = self._row(keep, promptLengths, "promptLengths", rows, IDS, logits)
-            p_rep = self._row(keep, repetition, "repetition", rows, FLOATS, logits)
-            p_pres = self._row(keep, presence, "presence", rows, FLOATS, logits)
-            p_freq = self._row(keep, frequency, "frequency", rows, FLOATS, logits)
+            p_history, history_stride, room = table_of(history, "history", at, IDS, rows)
+            p_lengths = self._row(keep, lengths, "lengths", shape, IDS)
+            p_prompt = self._row(keep, promptLengths, "promptLengths", shape, IDS)
+            p_rep = self._row(keep, repetition, "repetition", shape, FLOATS)
+            p_pres = self._row(keep, presence, "presence", shape, FLOATS)
+            p_freq = self._row(keep, frequency, "frequency", shape, FLOATS)
             if not room:
                 p_history = p_lengths = p_prompt = p_rep = p_pres = p_freq = None
         elif not (lengths is None and promptLengths is None and repetition is None and presence is None and frequency is None):
@@ -114,29 +117,28 @@ class TokenSampler:
         if biasTokens is not None or biases is not None:
             if biasTokens is None or biases is None:
                 raise ValueError("biasTokens and biases: one without the other")
-            p_ids = table_of(biasTokens, "biasTokens", at, IDS, rows)
-            n_bias, bias_stride = biasTokens.size(1), biasTokens.stride(0)
+            p_ids, bias_stride, n_bias = table_of(biasTokens, "biasTokens", at, IDS, rows)
             if n_bias > MAX_BIASES:
                 raise ValueError(f"biasTokens: at most {MAX_BIASES:,} a row")
-            p_biases = table_of(biases, "biases", at, FLOATS, rows)
-            if biases.size(1) != n_bias:
+            p_biases, other, n = table_of(biases, "biases", at, FLOATS, rows)
+            if n != n_bias:
                 raise ValueError(f"biases: shape {tuple(biases.shape)} where {(rows, n_bias)} is needed")
-            if biases.stride(0) != bias_stride and rows > 1 and n_bias:
+            if other != bias_stride and rows > 1 and n_bias:
                 raise ValueError("biases: another distance between rows than biasTokens")
         if mask is not None:
-            p_mask = table_of(mask, "mask", at, IDS, None)
-            mask_rows, mask_stride = mask.size(0), mask.stride(0)
-            if mask.size(1) < (self.vocabSize + 31) >> 5:
-                raise ValueError(f"mask: {mask.shape[1]} words, the vocabulary needs {(self.vocabSize + 31) // 32}")
+            p_mask, mask_stride, words = table_of(mask, "mask", at, IDS, None)
+            mask_rows = mask.shape[0]
+            if words < (self.vocabSize + 31) >> 5:
+                raise ValueError(f"mask: {words} words, the vocabulary needs {(self.vocabSize + 31) // 32}")
             if maskRows is not None:
-                p_which = row_of(maskRows, "maskRows", at, IDS, rows)
+                p_which = row_of(maskRows, "maskRows", at, IDS, shape)
                 if rows and not mask_rows:
                     raise ValueError("mask: no rows")
             elif mask_rows != rows:
                 raise ValueError(f"mask: {mask_rows} rows for {rows} rows of logits, and no maskRows")
         elif maskRows is not None:
             raise ValueError("maskRows: needs a mask")
-        return _lib.Logits(LOGITS_BYTES, LOGITS[logits.dtype], rows, n_bias, p_logits, logits.stride(0), p_history, history_stride, p_lengths, p_prompt,
+        return _lib.Logits(LOGITS_BYTES, LOGITS[logits.dtype], rows, n_bias, p_logits, row_stride, p_history, history_stride, p_lengths, p_prompt,
                            room, mask_rows, p_rep, p_pres, p_freq, p_ids, p_biases, bias_stride, p_mask, mask_stride, p_which)
 
     def adjustLogits(self, logits, out=None, history=None, lengths=None, promptLengths=None, repetition=None, presence=None, frequency=None,
@@ -152,14 +154,14 @@ class TokenSampler:
         p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
         if out is None:
             out = logits.new_empty((logits.size(0), self.vocabSize))
-        address = table_of(out, "out", self._engine.device_index, LOGITS, logits.size(0))
+        address, stride, columns = table_of(out, "out", self._engine.device_index, LOGITS, p.n_rows)
         if out.dtype != logits.dtype:
             raise ValueError(f"out: a tensor of {logits.dtype} is needed")
-        if out.size(1) < self.vocabSize:
-            raise ValueError(f"out: {out.size(1)} columns, the vocabulary has {self.vocabSize} tokens")
-        if out.stride(0) < self.vocabSize and out.size(0) > 1:
+        if columns < self.vocabSize:
+            raise ValueError(f"out: {columns} columns, the vocabulary has {self.vocabSize} tokens")
+        if stride < self.vocabSize and p.n_rows > 1:
             raise ValueError("out: rows overlap")
-        status = _lib.lib().b200bpe_sampler_adjust(self._h, C.byref(p), address, out.stride(0), raw_stream(self._engine.device_index))
+        status = _lib.lib().b200bpe_sampler_adjust(self._h, C.byref(p), address, stride, raw_stream(self._engine.device_index))
         if status:
             _lib.check(status, "b200bpe_sampler_adjust")
         return out
@@ -175,18 +177,18 @@ class TokenSampler:
         where the largest is taken).  A row without an allowed token gives -1 and -inf; a NaN is never chosen."""
         keep = []
         p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
-        rows = logits.size(0)
+        shape = logits.shape[:1]
         p_uniform = p_warm = p_k = p_p = p_m = None
         if uniform is not None:
-            p_uniform = row_of(uniform, "uniform", self._engine.device_index, FLOATS, rows)
-            p_warm = self._row(keep, temperature, "temperature", rows, FLOATS, logits)
-            p_k = self._row(keep, topK, "topK", rows, IDS, logits)
-            p_p = self._row(keep, topP, "topP", rows, FLOATS, logits)
-            p_m = self._row(keep, minP, "minP", rows, FLOATS, logits)
+            p_uniform = row_of(uniform, "uniform", self._engine.device_index, FLOATS, shape)
+            p_warm = self._row(keep, temperature, "temperature", shape, FLOATS)
+            p_k = self._row(keep, topK, "topK", shape, IDS)
+            p_p = self._row(keep, topP, "topP", shape, FLOATS)
+            p_m = self._row(keep, minP, "minP", shape, FLOATS)
         elif not (temperature is None and topK is None and topP is None and minP is None):
             raise ValueError("uniform: needed to draw")
         import torch
-        tokens, logprobs = logits.new_empty(rows, dtype=torch.int32), logits.new_empty(rows, dtype=torch.float32)
+        tokens, logprobs = logits.new_empty(shape, dtype=torch.int32), logits.new_empty(shape, dtype=torch.float32)
         c = _lib.Choice(CHOICE_BYTES, 0, p_uniform, p_warm, p_k, p_p, p_m, tokens.data_ptr(), logprobs.data_ptr())
         status = _lib.lib().b200bpe_sampler_sample(self._h, C.byref(p), C.byref(c), raw_stream(self._engine.device_index))
         if status:
