@@ -464,6 +464,9 @@ struct Kept {
 struct Draw { uint32_t owner; double base, target, near; };      // (owner 0xFFFFFFFF: not known)
 struct Best { float m, n; uint32_t at, pad; double sum; float cut[4]; };       // a CTA's part of what the first exchange brings
 
+// What a row's first exchange comes to: the sum of all weights in two units and the second in the first, the weights' exponent, and see there.
+struct Row { double quick_all, all, unit, steps; float from; bool quick; };
+
 struct Shared {
     Best best[SM_MAX_CLUSTER];
     double part_warp[2][SM_WARPS], part_cta[2][2][SM_MAX_CLUSTER];      // (the second index: one exchange and the next)
@@ -472,6 +475,7 @@ struct Shared {
     uint32_t border[2], again, candidates, quick_candidates, flag, place, at, cut_at[2];
     Kept kept;
     Draw draw;
+    Row row;
     union {
         uint32_t bins[SM_BINS];
         unsigned long long list[SM_CANDIDATES];      // candidates: key << 32 | ~token
@@ -1070,7 +1074,6 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
 
     // The first exchange: the largest x and the lowest token that has it, the sum of all weights, and for top_k a value that so many are not below.
     float m, n;
-    double all;
     for (bool again = false;; again = true) {
         m = value_of(__reduce_max_sync(0xFFFFFFFFu, key_of(stats.m)));
         n = stats.base(m);
@@ -1152,17 +1155,52 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         return;
     }
     if (set.greedy && (t.rank != 0 || t.warp != 0)) return;
-    const Weights w{m, stats.c, n, 64 * 1.4426950408889634 / set.warm, s.table};
-    const double unit = w.to_largest();
-    all = warp_sum(t.lane < t.C ? s.best[t.lane].sum * Stats::power(s.best[t.lane].n - n) : 0.0);
-    const double quick_all = all;
+    // What all warps need to know of the row; one works it out.
+    if (t.warp == 0) {
+        Row r;
+        const Weights w{m, stats.c, n, 0.0, nullptr};
+        r.unit = w.to_largest();
+        r.quick_all = warp_sum(t.lane < t.C ? s.best[t.lane].sum * Stats::power(s.best[t.lane].n - n) : 0.0);
+        r.all = r.quick_all * r.unit;
+        r.steps = set.greedy ? 0.0 : 64 * 1.4426950408889634 / set.warm;
+        // A value that all of the top_k, or all that top_p keeps, are not below, if there is such a one.
+        r.from = -INFINITY;
+        r.quick = quick_k;
+        if (quick_k) {
+            // At least top_k x are not below the largest value that 2^l of the CTAs have 1/2^l of top_k for.
+            for (uint32_t i = t.lane; i < 4 * SM_MAX_CLUSTER; i += 32) {
+                const uint32_t l = i / SM_MAX_CLUSTER, c = i % SM_MAX_CLUSTER;
+                if (c < t.C && 1u << l <= t.C) {
+                    const float mine = s.best[c].cut[l];
+                    uint32_t so_many = 0;
+                    for (uint32_t o = 0; o < t.C; o++) so_many += s.best[o].cut[l] >= mine;
+                    if (so_many >= 1u << l) r.from = fmaxf(r.from, mine);
+                }
+            }
+            r.from = value_of(__reduce_max_sync(0xFFFFFFFFu, key_of(r.from)));
+        } else if (quick_p) {
+            // What the CTAs' parts of 64, or of 256, weigh is enough.
+            for (int l = 0; l < 2 && !r.quick; l++) {
+                const double weight = warp_sum(t.lane < t.C ? (double)s.best[t.lane].cut[2 + l] * Stats::power(s.best[t.lane].n - n) : 0.0) * r.unit;
+                r.quick = weight >= (double)set.top_p * r.all;
+                r.from = value_of(__reduce_min_sync(0xFFFFFFFFu, t.lane < t.C ? key_of(s.best[t.lane].cut[l]) : 0xFFFFFFFFu));
+            }
+        }
+        if (t.lane == 0) s.row = r;
+    }
+    if (set.greedy) __syncwarp();
+    else __syncthreads();
+    const Weights w{m, stats.c, n, s.row.steps, s.table};
+    const double unit = s.row.unit, all = s.row.all;
+    const bool quick = s.row.quick;
+    float from = s.row.from;
     auto answer = [&](uint32_t token, float x) {
         how.tokens_out[sl.row] = token;
         if (how.logprobs_out)
-            how.logprobs_out[sl.row] = (float)(((double)x - (double)m) / set.warm - (log(quick_all) + 0.693147180559945309 * w.power_of_largest()));
+            how.logprobs_out[sl.row] = (float)(((double)x - (double)m) / set.warm - (log(s.row.quick_all) + 0.693147180559945309 * w.power_of_largest()));
     };
     if (set.greedy) {
-        if (t.rank == 0 && threadIdx.x == 0) {
+        if (threadIdx.x == 0) {
             uint32_t token = 0xFFFFFFFFu;
             for (uint32_t c = 0; c < t.C; c++)
                 if (s.best[c].m == m) token = min(token, s.best[c].at);
@@ -1170,34 +1208,10 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         }
         return;
     }
-    all *= unit;
 
     // The kept tokens.
     Kept kept{LOWEST_KEY, 0u};
     Draw draw{0xFFFFFFFFu, 0.0, 0.0, 0.0};
-    // Values that all of the top_k, or all that top_p keeps, are not below.
-    float from = -INFINITY;
-    bool quick = quick_k;
-    if (quick_k) {
-        // At least top_k x are not below the largest value that 2^l of the CTAs have 1/2^l of top_k for.
-        for (uint32_t i = t.lane; i < 4 * SM_MAX_CLUSTER; i += 32) {
-            const uint32_t l = i / SM_MAX_CLUSTER, c = i % SM_MAX_CLUSTER;
-            if (c < t.C && 1u << l <= t.C) {
-                const float mine = s.best[c].cut[l];
-                uint32_t so_many = 0;
-                for (uint32_t o = 0; o < t.C; o++) so_many += s.best[o].cut[l] >= mine;
-                if (so_many >= 1u << l) from = fmaxf(from, mine);
-            }
-        }
-        from = value_of(__reduce_max_sync(0xFFFFFFFFu, key_of(from)));
-    } else if (quick_p) {
-        // What the CTAs' parts of 64, or of 256, weigh is enough.
-        for (int l = 0; l < 2 && !quick; l++) {
-            const double weight = warp_sum(t.lane < t.C ? (double)s.best[t.lane].cut[2 + l] * Stats::power(s.best[t.lane].n - n) : 0.0) * unit;
-            quick = weight >= (double)set.top_p * all;
-            from = value_of(__reduce_min_sync(0xFFFFFFFFu, t.lane < t.C ? key_of(s.best[t.lane].cut[l]) : 0xFFFFFFFFu));
-        }
-    }
     if (quick) {
         from = fmaxf(from, -3.402823466e38f);            // (-infinity is never chosen)
         Shared* lead = t.peer(0);
