@@ -118,12 +118,12 @@ struct Span {
 template <uint32_t MOST>
 struct Special {
     uint32_t any[MOST / 32 + 1];         // masked, or in the history
-    uint32_t seen[MOST / 32 + 1];        // in the history: the buffer has its x (-infinity if it is masked)
+    uint32_t seen[MOST / 32 + 1];        // in the history, or with a bias: the buffer has its x (-infinity if it is masked)
     uint32_t todo[MOST / 32 + 1];        // not yet, it has its marks
 };
 
-// Makes `special`, and x of the places in the history: there, penalties cost a scattered load a token, not a test and a division for every lane of
-// the row.  Returns whether there are any special places.  Called by all threads of the CTA; ends with a barrier.
+// Makes `special`, and x of the places in the history and of those with a bias: so these cost a scattered load a token, not a test and a division for
+// every lane of the row.  Returns whether there are any special places.  Called by all threads of the CTA; ends with a barrier.
 // Each CTA reads the whole history of its row, and counts what is its own: a history is short beside a row, and L2 has it.  What a thread reads first
 // does not depend on anything else that is read, so that a row's settings and the first of its history are one wait.
 template <uint32_t MOST, class T>
@@ -143,7 +143,7 @@ __device__ __forceinline__ bool find_special(const b200bpe_logits& in, uint32_t 
         for (int k = 0; k < EACH; k++) t[k] = threadIdx.x + k * SM_THREADS < in.history_cap ? h[threadIdx.x + k * SM_THREADS] : 0u;
         if (pen.repetition == 1.0f && pen.presence == 0.0f && pen.frequency == 0.0f) n_seen = 0;
     }
-    if (n_seen == 0 && !mask.words && !mask.none) return false;
+    if (n_seen == 0 && in.n_bias == 0 && !mask.words && !mask.none) return false;
     const uint32_t words = (s.padded + 31u) / 32u, mask_words = (vocab + 31u) / 32u;
     for (uint32_t i = threadIdx.x; i < words; i += SM_THREADS) {
         uint32_t allowed = mask.none ? 0u : 0xFFFFFFFFu;
@@ -197,10 +197,29 @@ __device__ __forceinline__ bool find_special(const b200bpe_logits& in, uint32_t 
         }
         __syncthreads();
     }
+    if (in.n_bias) {
+        // Place i of the list takes all biases of its token, unless an earlier place has that token.
+        const uint32_t* list = in.bias_tokens + (uint64_t)s.row * in.bias_stride;
+        const float* by = in.biases + (uint64_t)s.row * in.bias_stride;
+        for (uint32_t i = threadIdx.x; i < in.n_bias; i += SM_THREADS) {
+            const uint32_t v = list[i], at = v - s.lo, p = at + s.lead, bit = 1u << (p & 31u);
+            if (at >= s.len || !mask.allows(v)) continue;
+            bool first = true;
+            for (uint32_t j = 0; j < i; j++) first &= list[j] != v;
+            if (!first) continue;
+            float x = __fadd_rn(special.seen[p >> 5] & bit ? s.buf[p] : as_float(row[at]), by[i]);
+            for (uint32_t j = i + 1; j < in.n_bias; j++)
+                if (list[j] == v) x = __fadd_rn(x, by[j]);
+            s.buf[p] = x;
+            atomicOr(&special.any[p >> 5], bit);
+            atomicOr(&special.seen[p >> 5], bit);
+        }
+        __syncthreads();
+    }
     return true;
 }
 
-// Calls to(place, N adjusted logits but for the biases) for the slice.  The first loads are the caller's (`ahead`, of first_loads): they are on their
+// Calls to(place, N adjusted logits) for the slice.  The first loads are the caller's (`ahead`, of first_loads): they are on their
 // way while special places are found, and a call with one row waits for little else.
 constexpr uint32_t SM_AHEAD = 4;
 template <class T>
@@ -257,24 +276,6 @@ __device__ __forceinline__ void store(float* at, const float (&v)[N]) {
     for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(at + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
 }
 
-// Adds the row's biases to the slice's x.  Called by all threads of the CTA, with a barrier in front; one has to follow.
-__device__ __forceinline__ void add_biases(const b200bpe_logits& in, const Slice& s, const MaskRow& mask) {
-    // Place i takes all biases of its token, unless an earlier place has that token.
-    const uint32_t* list = in.bias_tokens + (uint64_t)s.row * in.bias_stride;
-    const float* by = in.biases + (uint64_t)s.row * in.bias_stride;
-    for (uint32_t i = threadIdx.x; i < in.n_bias; i += SM_THREADS) {
-        const uint32_t t = list[i];
-        if (t < s.lo || t - s.lo >= s.len || !mask.allows(t)) continue;
-        bool first = true;
-        for (uint32_t j = 0; j < i; j++) first &= list[j] != t;
-        if (!first) continue;
-        float v = __fadd_rn(s.buf[s.lead + t - s.lo], by[i]);
-        for (uint32_t j = i + 1; j < in.n_bias; j++)
-            if (list[j] == t) v = __fadd_rn(v, by[j]);
-        s.buf[s.lead + t - s.lo] = v;
-    }
-}
-
 // Slice `part` of row `row`, of `whole` tokens but for the last ones.
 template <class T>
 __device__ __forceinline__ Slice slice_of(const b200bpe_logits& in, uint32_t vocab, uint32_t row, uint32_t part, uint32_t whole, float* buf) {
@@ -308,7 +309,7 @@ __device__ __forceinline__ void write_out(T* to, const Slice& s, bool alike, uin
     }
 }
 
-// A CTA for each slice of a row.  Bound by memory: a row is read and written once; only with biases does x pass through shared memory.
+// A CTA for each slice of a row.  Bound by memory: a row is read and written once, and its special places are few.
 template <class T>
 __global__ void __launch_bounds__(SM_THREADS, 4)
 k_adjust(const __grid_constant__ b200bpe_logits in, uint32_t vocab, T* out, uint64_t out_stride) {
@@ -324,21 +325,7 @@ k_adjust(const __grid_constant__ b200bpe_logits in, uint32_t vocab, T* out, uint
     T* to = out + (uint64_t)s.row * out_stride + s.lo;
     // Places that lie on 16 bytes in the logits do so in the output if its rows are aligned like the logits' (in place, and with equal strides).
     const bool alike = (reinterpret_cast<uint64_t>(to) & 15u) == s.lead * sizeof(T);
-    constexpr uint32_t N = Packed<T>::N;
-    if (!in.n_bias) {
-        each_adjusted(row, s, ahead, any_special, special, [&](uint32_t p, float (&v)[N]) { write_out<T>(to, s, alike, p, v); });
-        return;
-    }
-    each_adjusted(row, s, ahead, any_special, special, [&](uint32_t p, float (&v)[N]) { store(buf + p, v); });
-    __syncthreads();
-    add_biases(in, s, mask);
-    __syncthreads();
-    for (uint32_t p = threadIdx.x * N; p < s.padded; p += SM_THREADS * N) {
-        float v[N];
-#pragma unroll
-        for (uint32_t k = 0; k < N; k++) v[k] = buf[p + k];
-        write_out<T>(to, s, alike, p, v);
-    }
+    each_adjusted(row, s, ahead, any_special, special, [&](uint32_t p, float (&v)[Packed<T>::N]) { write_out<T>(to, s, alike, p, v); });
 }
 
 // ── the choice ──
@@ -1062,14 +1049,8 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         const bool any_special = find_special(in, vocab, row, sl, mask, s.special);
         each_adjusted(row, sl, ahead, any_special, s.special, [&](uint32_t p, float (&v)[Packed<T>::N]) {
             store(buf + p, v);
-            if (!in.n_bias) stats.add(v, p, buf);
+            stats.add(v, p, buf);
         });
-        if (in.n_bias) {
-            __syncthreads();
-            add_biases(in, sl, mask);
-            __syncthreads();
-            slice_stats(sl, stats);
-        }
     }
 
     // The first exchange: the largest x and the lowest token that has it, the sum of all weights, and for top_k a value that so many are not below.
