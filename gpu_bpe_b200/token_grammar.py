@@ -80,7 +80,7 @@ class TokenGrammar:
         p_states, p_tokens = row_of(states, "states", at, IDS, shape), row_of(tokens, "tokens", at, IDS, shape)
         if out is None:
             import torch
-            out = states.new_empty(shape, dtype=torch.int32)
+            out = states.new_empty(rows, dtype=torch.int32)
             p_out = out.data_ptr()
         else:
             p_out = row_of(out, "out", at, IDS, shape)
@@ -95,7 +95,7 @@ class TokenGrammar:
                 raise ValueError("history: rows overlap")
             if lengthsOut is None:
                 import torch
-                lengthsOut = lengths.new_empty(shape, dtype=torch.int32)
+                lengthsOut = lengths.new_empty(rows, dtype=torch.int32)
                 p_new = lengthsOut.data_ptr()
             else:
                 p_new = row_of(lengthsOut, "lengthsOut", at, IDS, shape)

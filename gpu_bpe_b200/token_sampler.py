@@ -188,7 +188,7 @@ class TokenSampler:
         elif not (temperature is None and topK is None and topP is None and minP is None):
             raise ValueError("uniform: needed to draw")
         import torch
-        tokens, logprobs = logits.new_empty(shape, dtype=torch.int32), logits.new_empty(shape, dtype=torch.float32)
+        tokens, logprobs = logits.new_empty(p.n_rows, dtype=torch.int32), logits.new_empty(p.n_rows, dtype=torch.float32)
         c = _lib.Choice(CHOICE_BYTES, 0, p_uniform, p_warm, p_k, p_p, p_m, tokens.data_ptr(), logprobs.data_ptr())
         status = _lib.lib().b200bpe_sampler_sample(self._h, C.byref(p), C.byref(c), raw_stream(self._engine.device_index))
         if status:
