@@ -472,21 +472,24 @@ struct Shared {
     Row row;
     union {
         uint32_t bins[SM_BINS];
-        unsigned long long list[SM_CANDIDATES];      // candidates: key << 32 | ~token
+        unsigned long long __align__(16) list[SM_CANDIDATES];      // candidates: key << 32 | ~token
         uint32_t keys[SM_THREADS];
         Special<SM_MAX_SLICE + 8> special;           // until the slice is there
     };
 };
 
-__device__ __forceinline__ double warp_sum(double v) {
+// Over a warp, or over each N lanes of it.
+template <int N = 32, class V>
+__device__ __forceinline__ V warp_sum(V v) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    for (int o = N / 2; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     return v;
 }
-__device__ __forceinline__ double warp_run(double v, int lane) {        // over the lanes up to this one
+template <int N = 32, class V>
+__device__ __forceinline__ V warp_run(V v, int lane) {        // over the lanes up to this one, of the first N
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    for (int o = 1; o < N; o <<= 1) {
+        const V y = __shfl_up_sync(0xFFFFFFFFu, v, o);
         if (lane >= o) v += y;
     }
     return v;
@@ -519,8 +522,8 @@ struct Team {
         __syncthreads();
         par ^= 1;
         if (warp == 0) {
-            a = warp_sum(lane < SM_WARPS ? s.part_warp[0][lane] : 0.0);
-            b = warp_sum(lane < SM_WARPS ? s.part_warp[1][lane] : 0.0);
+            a = warp_sum<SM_WARPS>(s.part_warp[0][lane % SM_WARPS]);
+            b = warp_sum<SM_WARPS>(s.part_warp[1][lane % SM_WARPS]);
             if (lane < C) {
                 Shared* p = peer(lane);
                 p->part_cta[0][par][rank] = a;
@@ -528,29 +531,30 @@ struct Team {
             }
         }
         sync();
-        a = warp_sum(lane < C ? part(0, lane) : 0.0);
-        b = warp_sum(lane < C ? part(1, lane) : 0.0);
+        a = of_ctas(part(0, lane % SM_MAX_CLUSTER));
+        b = of_ctas(part(1, lane % SM_MAX_CLUSTER));
     }
+    // Sum of what lanes have for CTA `lane % SM_MAX_CLUSTER`.
+    __device__ double of_ctas(double v) const { return warp_sum<SM_MAX_CLUSTER>(lane % SM_MAX_CLUSTER < C ? v : 0.0); }
     __device__ double part(int i, uint32_t cta) const { return s.part_cta[i][par][cta]; }
 
     // Sum of v over the threads before this one; *all: over all.
-    __device__ double before(double v, double* all) {
-        const double run = warp_run(v, lane);
+    template <class V>
+    __device__ V before(V v, V* all) {
+        V* part = reinterpret_cast<V*>(s.scan_warp);
+        const V run = warp_run(v, lane);
         __syncthreads();
-        if (lane == 31) s.scan_warp[warp] = run;
+        if (lane == 31) part[warp] = run;
         __syncthreads();
-        double base = 0, sum = 0;
-#pragma unroll
-        for (int w = 0; w < SM_WARPS; w++) {
-            if (w == warp) base = sum;
-            sum += s.scan_warp[w];
-        }
-        *all = sum;
-        return base + run - v;
+        const V sums = warp_run<SM_WARPS>(part[lane % SM_WARPS], lane % SM_WARPS);
+        *all = __shfl_sync(0xFFFFFFFFu, sums, SM_WARPS - 1);
+        const V base = __shfl_sync(0xFFFFFFFFu, sums, warp - 1);
+        return (warp ? base : V(0)) + run - v;
     }
-    // The first of n values (a lane's is v) at which the running sum is above target, and the sum in front of it; if there is none, the last above 0.
+    // The first of N values (a lane's is v; 0 behind the first N lanes) at which the running sum is above target, and the sum in front of it; if there is none, the last above 0.
+    template <int N = 32>
     __device__ int first_above(double v, double from, double target, double* base) const {
-        const double run = from + warp_run(v, lane);
+        const double run = from + warp_run<N>(v, lane);
         const uint32_t above = __ballot_sync(0xFFFFFFFFu, v > 0 && run > target), some = __ballot_sync(0xFFFFFFFFu, v > 0);
         const int i = above ? __ffs(above) - 1 : some ? 31 - __clz(some) : 0;
         *base = __shfl_sync(0xFFFFFFFFu, run - v, i);
@@ -586,49 +590,58 @@ __device__ __forceinline__ double kept_mass(const Slice& sl, int warp, const Wei
 
 // The first place of the slice at which base plus the running sum of f(place, x) is above target; if there is none, the last with f above 0.  Every
 // warp's sum of f is in s.warp_mass.  *near: whether a sum that decided was within `margin` of target (or the sums of parts and of places round apart).
-// Called by all threads of one CTA: first the part of a warp, then a step of 128 places of it, then a place.
-template <class F>
+// Called by all threads of one CTA: first the part of a warp, then a step of 128 places of it, then a place.  f gives V.
+template <class V, class F>
 __device__ uint32_t find_place(Team& t, const Slice& sl, double base, double target, double margin, bool* near, F f) {
     static_assert(SM_MAX_SLICE + 8 <= SM_WARPS * 32 * 128, "more than 32 steps in a warp's part");
+    constexpr int EACH = 32 / SM_WARPS;
     Shared& s = t.s;
-    const float4 nothing = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    const Span span(sl.padded, t.first_above(t.lane < SM_WARPS ? s.warp_mass[t.lane] : 0.0, base, target, &base));
-    for (uint32_t i = t.warp; i < 32; i += SM_WARPS) {
-        const uint32_t p = span.lo + i * 128 + t.lane * 4;
-        double v = 0;
-        if (span.lo + i * 128 < span.hi) {
-            const float4 x = p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : nothing;
-            v = warp_sum((f(p, x.x) + f(p + 1, x.y)) + (f(p + 2, x.z) + f(p + 3, x.w)));
+    const Span span(sl.padded, t.first_above<SM_WARPS>(t.lane < SM_WARPS ? s.warp_mass[t.lane] : 0.0, base, target, &base));
+    // A warp has EACH of the steps, a lane four neighbouring places of each.
+    V v[EACH][4], run[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const uint32_t at = span.lo + (i * SM_WARPS + t.warp) * 128, p = at + t.lane * 4;
+        run[i] = v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0;
+        if (at < span.hi) {
+            const float4 x = p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            v[i][0] = f(p, x.x);
+            v[i][1] = f(p + 1, x.y);
+            v[i][2] = f(p + 2, x.z);
+            v[i][3] = f(p + 3, x.w);
+            run[i] = warp_run((v[i][0] + v[i][1]) + (v[i][2] + v[i][3]), t.lane);
         }
-        if (t.lane == 0) s.step_mass[i] = v;
+        if (t.lane == 31) s.step_mass[i * SM_WARPS + t.warp] = (double)run[i];
     }
+    if (threadIdx.x == 0) { s.place = 0u; s.flag = 1u; }
     __syncthreads();
-    if (t.warp == 0) {
-        const int step = t.first_above(s.step_mass[t.lane], base, target, &base);
-        const uint32_t p = span.lo + step * 128 + t.lane * 4;
-        const float4 x = p < span.hi ? *reinterpret_cast<const float4*>(sl.buf + p) : nothing;
-        const double v[4] = {f(p, x.x), f(p + 1, x.y), f(p + 2, x.z), f(p + 3, x.w)}, mine = (v[0] + v[1]) + (v[2] + v[3]);
-        double sum = base + warp_run(mine, t.lane) - mine;
+    const double mass = s.step_mass[t.lane];
+    const int step = t.first_above(mass, base, target, &base);
+    if (step % SM_WARPS == t.warp) {
+        const double whole = __shfl_sync(0xFFFFFFFFu, mass, step);
+        if (sizeof(V) == 4) margin += whole * (10.0 / 16777216);          // (within a step: a product, the sums of four, five steps of a scan, two differences)
         uint32_t hit = 0, last = 0;
         bool edge = false;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const double next = sum + v[k];
-            if (v[k] > 0) {
-                last = p + k + 1;
-                if (hit == 0) {
-                    edge = fabs(next - target) <= margin || fabs(sum - target) <= margin;
-                    if (next > target) hit = p + k + 1;
+        for (int i = 0; i < EACH; i++) {
+            if (i * SM_WARPS + t.warp != step) continue;
+            const uint32_t p = span.lo + step * 128 + t.lane * 4;
+            double sum = base + (double)(run[i] - ((v[i][0] + v[i][1]) + (v[i][2] + v[i][3])));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const double next = sum + (double)v[i][k];
+                if (v[i][k] > 0) {
+                    last = p + k + 1;
+                    if (hit == 0) {
+                        edge = fabs(next - target) <= margin || fabs(sum - target) <= margin;
+                        if (next > target) hit = p + k + 1;
+                    }
                 }
+                sum = next;
             }
-            sum = next;
         }
         const uint32_t above = __ballot_sync(0xFFFFFFFFu, hit != 0), some = __ballot_sync(0xFFFFFFFFu, last != 0);
-        const int l = above ? __ffs(above) - 1 : some ? 31 - __clz(some) : 0;
-        hit = __shfl_sync(0xFFFFFFFFu, hit, l);
-        last = __shfl_sync(0xFFFFFFFFu, last, l);
-        edge = __shfl_sync(0xFFFFFFFFu, edge, l);
-        if (t.lane == 0) {
+        if (t.lane == (above ? __ffs(above) - 1 : some ? 31 - __clz(some) : 0)) {
             s.place = (above ? hit : some ? last : 1u) - 1u;
             s.flag = edge || !above;
         }
@@ -679,13 +692,34 @@ __device__ __forceinline__ void sort_threads(unsigned long long* list) {
     for (int k = 0; k < E; k++) list[i0 + k] = a[k];
     __syncthreads();
 }
+// The same of at most SM_THREADS / 2 numbers, all unlike but for zeros behind them: each is put where as many as are larger lie in front.  (For 128 that is
+// a third of the instructions of a network; for 256 it would be more.)
+__device__ __forceinline__ void sort_few(unsigned long long* list, uint32_t n) {
+    uint32_t size = 32;
+    while (size < n) size *= 2;
+    const uint32_t shares = SM_THREADS / size, e = threadIdx.x / shares, part = threadIdx.x % shares;
+    const unsigned long long mine = list[e];
+    uint32_t rank = 0;
+#pragma unroll 4
+    for (uint32_t j = part * 2; j < size; j += shares * 2) {
+        const ulonglong2 other = *reinterpret_cast<const ulonglong2*>(list + j);
+        rank += (other.x > mine) + (other.y > mine);
+    }
+    for (uint32_t o = 1; o < shares; o *= 2) rank += __shfl_xor_sync(0xFFFFFFFFu, rank, o);
+    __syncthreads();
+    if (part == 0 && mine) list[rank] = mine;
+    const uint32_t full = __syncthreads_count(part == 0 && mine != 0ull);
+    if (part == 0 && e >= full) list[e] = 0ull;
+    __syncthreads();
+}
 // Of n numbers (zeros behind them are added); returns how many lie at a thread: thread i has those from i * that on.
 __device__ __forceinline__ uint32_t sort_down(unsigned long long* list, uint32_t n) {
     const uint32_t size = n <= SM_THREADS ? SM_THREADS : n <= 2 * SM_THREADS ? 2 * SM_THREADS : 4 * SM_THREADS;
     static_assert(SM_CANDIDATES == 4 * SM_THREADS, "the list's room");
     for (uint32_t i = n + threadIdx.x; i < size; i += SM_THREADS) list[i] = 0ull;
     __syncthreads();
-    if (size == SM_THREADS) sort_threads<1>(list);
+    if (n <= SM_THREADS / 2) sort_few(list, n);
+    else if (size == SM_THREADS) sort_threads<1>(list);
     else if (size == 2 * SM_THREADS) sort_threads<2>(list);
     else sort_threads<4>(list);
     return size / SM_THREADS;
@@ -697,16 +731,25 @@ struct Bins {
     __device__ Bins(float largest, double range) : m(largest), scale((float)(SM_BINS / fmin(range, 3.4e38))) {}
     static constexpr float MAGIC = 8388608.0f;       // added to 0 to 2^22, it leaves the nearest whole number in the lowest bits
     __device__ __forceinline__ float at(float x) const { return (m - x) * scale; }
-    // Puts x into its bin, if it lies in front of `end`: as 1, or as its weight in parts of 2^16 of that of its bin's middle, bins being 1/64 wide: e^-r by
-    // its first terms.
+    // Puts four x into their bins, as far as they lie in front of `end`: as 1, or as its weight in parts of 2^16 of that of its bin's middle, bins being 1/64
+    // wide: e^-r by its first terms.
     template <bool MASS>
-    __device__ __forceinline__ void put(uint32_t* bins, float x, float end) const {
-        const float a = at(x);
-        if (a < end) {
-            const float b = a + MAGIC, r = a - (b - MAGIC);
-            const uint32_t n = MASS ? __float_as_uint(fmaf(fmaf(r, 8.0f, -1024.0f), r, MAGIC + 65536.0f)) & 0x7FFFFFu : 1u;
-            atomicAdd(bins + (__float_as_uint(b) & 0x7FFFFFu), n);
+    __device__ __forceinline__ void put(uint32_t* bins, const float4& x, float end) const {
+        const float v[4] = {x.x, x.y, x.z, x.w};
+        float a[4], b[4];
+        uint32_t n[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) a[k] = at(v[k]);
+        if (fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) >= end) return;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            b[k] = fminf(a[k], end) + MAGIC;
+            const float r = a[k] - (b[k] - MAGIC);
+            n[k] = MASS ? __float_as_uint(fmaf(fmaf(r, 8.0f, -1024.0f), r, MAGIC + 65536.0f)) & 0x7FFFFFu : 1u;
         }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (a[k] < end) atomicAdd(bins + (__float_as_uint(b[k]) & 0x7FFFFFu), n[k]);
     }
     // A value that is above all x of the bins from `bin` on, or, `under`, below all x of the bins up to it: next to the bin's end, by more than `at` is off.
     __device__ float end_of(uint32_t bin, bool under) const {
@@ -787,7 +830,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     // every CTA adds up a part of the bins for all
     const uint32_t mine = SM_BINS / t.C, per = max(mine / SM_THREADS, 1u), first = t.rank * mine + threadIdx.x * per;
     const bool busy = threadIdx.x * per < mine;
-    double here[SM_BINS / SM_THREADS], sum = 0;
+    float here[SM_BINS / SM_THREADS], sum = 0;          // (the borders of bins are known to 2^-15 only)
 #pragma unroll
     for (uint32_t k = 0; k < SM_BINS / SM_THREADS; k++) {
         here[k] = 0;
@@ -795,22 +838,22 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
             unsigned long long n = 0;
 #pragma unroll 8
             for (uint32_t c = 0; c < t.C; c++) n += t.peer(c)->bins[first + k];
-            here[k] = MASS ? (double)((float)n * (__expf(-(float)(first + k) / 64) / 65536.0f)) : (double)n;
+            here[k] = MASS ? (float)n * (__expf(-(float)(first + k) / 64) / 65536.0f) : (float)n;
         }
         sum += here[k];
     }
     if (threadIdx.x < 2) s.border[threadIdx.x] = SM_BINS - 1;
     if (threadIdx.x == 0) s.candidates = 0u;
-    double all, at = t.before(sum, &all);
+    float all, before = t.before(sum, &all);
     // (t.total's barriers: the parts of a bin may be read until here)
-    double a = threadIdx.x == 0 ? all : 0.0, none = 0;
+    double a = threadIdx.x == 0 ? (double)all : 0.0, none = 0;
     t.total(a, none);
-    at += warp_sum(t.lane < t.rank ? t.part(0, t.lane) : 0.0);
+    double at = (double)before + warp_sum(t.lane < t.rank ? t.part(0, t.lane) : 0.0);
     const double slack = MASS ? 1.0 / 32768 : 0.0;          // 2^-17 a weight, 2 * 2^-24 * 2048 / 64 its place, the bins' weights, and what the target is off
 #pragma unroll
     for (uint32_t k = 0; k < SM_BINS / SM_THREADS; k++) {
         if (k >= per || !busy) break;
-        const double next = at + here[k];
+        const double next = at + (double)here[k];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             const double by = e == 0 ? 1.0 + slack : 1.0 - slack;
@@ -895,7 +938,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                     const double stay = warp_sum(part);
                     draw.target = (double)set->uniform * stay;
                     draw.near = how_near(vocab, stay, set->uniform, false);
-                    draw.owner = t.first_above(part, 0.0, draw.target, &draw.base);
+                    draw.owner = t.first_above<SM_MAX_CLUSTER>(part, 0.0, draw.target, &draw.base);
                 }
                 if (threadIdx.x < t.C) {
                     Shared* p = t.peer(threadIdx.x);
@@ -960,10 +1003,10 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     t.total(equal, none);
     if (ties >= equal) return Kept{least, 0xFFFFFFFFu};
     double base;
-    const uint32_t owner = t.first_above(t.lane < t.C ? t.part(0, t.lane) : 0.0, 0.0, ties - 0.5, &base);
+    const uint32_t owner = t.first_above<SM_MAX_CLUSTER>(t.lane < t.C ? t.part(0, t.lane) : 0.0, 0.0, ties - 0.5, &base);
     if (t.rank == owner) {
         bool near;
-        const uint32_t p = find_place(t, sl, base, ties - 0.5, 0.0, &near, [&](uint32_t, float x) { return key_of(x) == least ? 1.0 : 0.0; });
+        const uint32_t p = find_place<double>(t, sl, base, ties - 0.5, 0.0, &near, [&](uint32_t, float x) { return key_of(x) == least ? 1.0 : 0.0; });
         if (threadIdx.x < t.C) t.peer(threadIdx.x)->cut_at[1] = p + shift + 1u;
     }
     t.sync();
@@ -1118,7 +1161,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         __syncthreads();
         if (!again) cluster.barrier_wait();
         if (t.warp == 0) {
-            const Best b{m, n, s.at, 0u, warp_sum(t.lane < SM_WARPS ? s.part_warp[0][t.lane] * Stats::power(s.n_warp[t.lane] - n) : 0.0),
+            const Best b{m, n, s.at, 0u, warp_sum<SM_WARPS>(s.part_warp[0][t.lane % SM_WARPS] * Stats::power(s.n_warp[t.lane % SM_WARPS] - n)),
                          {s.cut[0], s.cut[1], s.cut[2], s.cut[3]}};
             if (t.lane < t.C) t.peer(t.lane)->best[t.rank] = b;
         }
@@ -1244,7 +1287,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         // (what weighs less than e^-32 does not matter to top_p; it may to top_k, where a temperature is low)
         const Bins bins(m, fmax(32.0 * set.warm, 24.0));
         each_four(sl, t.warp, [&](uint32_t, const float4& x) {
-            for (float v : {x.x, x.y, x.z, x.w}) bins.put<false>(s.bins, v, SM_BINS - 1.5f);
+            bins.put<false>(s.bins, x, SM_BINS - 1.5f);
         });
         t.sync();
         kept = border<false>(t, sl, w, bins, (double)set.top_k, -1.0, 0.0, nullptr, vocab, draw);
@@ -1264,7 +1307,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
             float end = SM_BINS - 1.5f;
             if (set.top_p < 0.999f) end = fminf(end, 64.0f * logf((float)((double)vocab / (0.5 * (1.0 - set.top_p) * whole))) + 1.0f);
             each_four(sl, t.warp, [&](uint32_t, const float4& x) {
-                for (float v : {x.x, x.y, x.z, x.w}) bins.put<true>(s.bins, v, end);
+                bins.put<true>(s.bins, x, end);
             });
             t.sync();
             k = border<true>(t, sl, w, bins, (double)set.top_p * whole, by_k ? -1.0 : (double)set.top_p, how_near(vocab, whole, set.top_p, by_k),
@@ -1285,9 +1328,8 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         constexpr bool EXACT = decltype(exact)::value;
         if (t.rank == draw.owner) {
             bool near;
-            *place = find_place(t, sl, draw.base, draw.target, EXACT ? 0.0 : draw.near, &near, [&](uint32_t p, float x) {
-                return kept.has(x, p + shift) ? (EXACT ? w.exact(x) : (double)w.quick(x) * unit) : 0.0;
-            });
+            if (EXACT) *place = find_place<double>(t, sl, draw.base, draw.target, 0.0, &near, [&](uint32_t p, float x) { return kept.has(x, p + shift) ? w.exact(x) : 0.0; });
+            else *place = find_place<float>(t, sl, draw.base, draw.target, draw.near, &near, [&](uint32_t p, float x) { return kept.has(x, p + shift) ? w.quick(x) * (float)unit : 0.0f; });
             if (!EXACT && threadIdx.x < t.C) t.peer(threadIdx.x)->cut_at[0] = near;
         }
         return t.rank == draw.owner;
@@ -1297,7 +1339,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         const double stay = warp_sum(part);
         d.target = (double)set.uniform * stay;
         d.near = how_near(vocab, stay, set.uniform, false);
-        d.owner = t.first_above(part, 0.0, d.target, &d.base);
+        d.owner = t.first_above<SM_MAX_CLUSTER>(part, 0.0, d.target, &d.base);
         return d;
     };
     if (draw.owner != 0xFFFFFFFFu) {
