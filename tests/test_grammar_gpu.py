@@ -209,3 +209,22 @@ def test_c_entry_points(engine, torch):
     assert bad(L.b200bpe_grammar_advance(g._h, t.data_ptr(), t.data_ptr(), 1, t.data_ptr(), t.data_ptr(), 1, 1, None, None, None))
     assert L.b200bpe_grammar_mask(g._h, None, 0, None, 0, None) == 0
     g.destroy()
+
+
+def test_masks_of_all_states_ahead(engine, torch):
+    """A grammar's masks made once, rows of a batch picked from them by state."""
+    rng = np.random.default_rng(4)
+    vocab = _vocabulary(rng, 900)
+    table, accepting = _automaton(rng, 60)
+    g, s = TokenGrammar(engine, vocab, table, accepting, 899), TokenSampler(engine, 900)
+    every = g.allowedTokens(torch.arange(60, dtype=torch.int32, device="cuda"))
+    states = torch.from_numpy(rng.integers(-1, 61, 40).astype(np.int32)).cuda()
+    logits, u = torch.randn(40, 900, device="cuda"), torch.rand(40, device="cuda")
+    direct, by_state = s.sample(logits, u, mask=g.allowedTokens(states)), s.sample(logits, u, mask=every, maskRows=states)
+    assert torch.equal(direct[0], by_state[0]) and torch.equal(direct[1], by_state[1])
+    ahead = g.advance(states, direct[0]).cpu().numpy()
+    for k, t, to in zip(states.cpu().numpy(), direct[0].cpu().numpy(), ahead):
+        ok = model.allowed(vocab, table, accepting, 899, k)
+        assert (t == -1 and not ok.any() and to == k) or (ok[t] and to >= 0)
+    g.destroy()
+    s.destroy()

@@ -365,3 +365,64 @@ def test_a_sampler_outlives_its_engine(torch):
     e.destroy()
     assert torch.equal(s.sample(t)[0], t.argmax(1).int())
     s.destroy()
+
+
+@pytest.mark.parametrize("length", [1, 255, 256, 2047, 2048, 2049, 5000])
+def test_lengths_of_a_history(engine, torch, length):
+    """Either side of what a thread keeps at hand; most of it one token, the rest spread over the vocabulary."""
+    vocab, rows = 40_000, 2
+    rng = np.random.default_rng(length)
+    s = TokenSampler(engine, vocab)
+    t, values = _logits(rng, rows, vocab, "bfloat16", torch)
+    history = np.where(rng.random((rows, length)) < 0.4, 17, rng.integers(0, vocab, (rows, length))).astype(np.int32)
+    e = dict(history=history, lengths=np.full(rows, length, np.int32), prompt=np.array([0, length // 3], np.int32), repetition=np.float32([1.4, 1]),
+             frequency=np.float32([0.01, 0.02]), presence=np.float32([0.3, 0]), mask=model.packed(rng.random((rows, vocab)) < 0.9))
+    x, bound = model.adjusted(values.astype(np.float64), np.float64, **e)
+    a = _arguments(torch, e)
+    _agree(x, bound, s.adjustLogits(t, **a).float().cpu().numpy(), "bfloat16")
+    x, _ = model.adjusted(values, np.float32, **e)
+    u, st = _settings(rng, rows, vocab)
+    _compare(x, *_sample(torch, s, t, u, st, **a), vocab, u, **st)
+    a["history"], a["lengths"] = a["history"].view(torch.uint32), a["lengths"].view(torch.uint32)
+    _compare(x, *_sample(torch, s, t, u, st, **a), vocab, u, **st)
+    s.destroy()
+
+
+def test_the_largest_vocabulary(engine, torch):
+    vocab, rows = 327_680, 3
+    rng = np.random.default_rng(10)
+    s = TokenSampler(engine, vocab)
+    t, values = _logits(rng, rows, vocab, "float16", torch)
+    u = rng.random(rows).astype(np.float32)
+    for st in ({}, {"k": np.array([3, 300, 100_000], np.int32)}, {"p": np.full(rows, 0.97, np.float32), "t": np.float32([0.3, 1, 1.5])}):
+        _compare(values, *_sample(torch, s, t, u, st), vocab, u, **st)
+    s.destroy()
+
+
+def test_one_row_for_all(engine, torch):
+    """Rows that lie on top of one another are only read."""
+    vocab, rows = 7000, 9
+    rng = np.random.default_rng(11)
+    s = TokenSampler(engine, vocab)
+    t, values = _logits(rng, 1, vocab, "float32", torch)
+    u = ((np.arange(rows) + 0.5) / rows).astype(np.float32)
+    x = np.repeat(values, rows, 0)
+    _compare(x, *_sample(torch, s, t.expand(rows, vocab), u), vocab, u)
+    assert torch.equal(s.adjustLogits(t.expand(rows, vocab)), t.expand(rows, vocab))
+    s.destroy()
+
+
+def test_draws_follow_the_weights(engine, torch):
+    """Uniforms on a grid draw each token as often as its share of the grid, to one."""
+    vocab, n = 3000, 20_000
+    rng = np.random.default_rng(12)
+    s = TokenSampler(engine, vocab)
+    t, values = _logits(rng, 1, vocab, "float32", torch)
+    u = (torch.arange(n, device="cuda") + 0.5) / n
+    tokens = s.sample(t.expand(n, vocab), u, topK=torch.full((n,), 40, dtype=torch.int32, device="cuda"))[0].cpu().numpy()
+    order = np.argsort(-values[0], kind="stable")[:40]
+    w = np.exp(values[0].astype(np.float64) - values[0].max())
+    share = np.zeros(vocab)
+    share[order] = w[order] / w[order].sum()
+    assert np.abs(np.bincount(tokens, minlength=vocab) - n * share).max() <= 1 and (np.diff(tokens) >= 0).all()
+    s.destroy()
