@@ -312,6 +312,7 @@ b200bpe_status b200bpe_grammar_mask(b200bpe_grammar* h, const uint32_t* states, 
     const GrammarTables& g = h->g.g;
     const uint32_t words = (g.entries + 31u) / 32u;
     if (!states || !mask_out) return refused("b200bpe_grammar_mask: null pointer");
+    if ((reinterpret_cast<uint64_t>(states) | reinterpret_cast<uint64_t>(mask_out)) % 4) return refused("b200bpe_grammar_mask: a misaligned pointer");
     if (mask_stride < words && n_rows > 1) return refused("b200bpe_grammar_mask: rows of the mask overlap");
     const OnDevice on(h->g.ctx->device);
     B2_CUDA(on.error);
@@ -337,6 +338,8 @@ b200bpe_status b200bpe_grammar_advance(b200bpe_grammar* h, const uint32_t* state
     if (n_rows >= 1u << 28) return refused("b200bpe_grammar_advance: more than 2^28 - 1 rows");
     if (n_rows == 0) return B200BPE_OK;
     if (!states || !tokens || !states_out) return refused("b200bpe_grammar_advance: null pointer");
+    for (const void* p : {(const void*)states, (const void*)tokens, (const void*)states_out, (const void*)history, (const void*)lengths, (const void*)lengths_out})
+        if (reinterpret_cast<uint64_t>(p) % 4) return refused("b200bpe_grammar_advance: a misaligned pointer");
     if (history && (!lengths || !lengths_out)) return refused("b200bpe_grammar_advance: a history without lengths");
     if (history && history_stride < history_cap && n_rows > 1) return refused("b200bpe_grammar_advance: rows of the history overlap");
     if (!history && (lengths || lengths_out)) return refused("b200bpe_grammar_advance: lengths without a history");

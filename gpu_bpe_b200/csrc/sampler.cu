@@ -1136,7 +1136,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         n = stats.base(m);
         if (stats.m == m && m > -INFINITY) {
             uint32_t p = stats.at;
-            while (buf[p] != m) p++;
+            for (int k = 1; k < Packed<T>::N && buf[p] != m; k++) p++;
             atomicMin(&s.at, p + shift);
         }
         if (t.warp < (quick_k ? 4 : quick_p ? 2 : 0)) {
@@ -1387,11 +1387,17 @@ struct Sampler {
     uint32_t vocab = 0;
 };
 
+// Whether these pointers to 32-bit values lie as such values have to.
+template <class... P>
+static bool words(const P*... p) { return (... && (reinterpret_cast<uint64_t>(p) % 4 == 0)); }
+
 static b200bpe_status check_logits(const b200bpe_logits* in) {
     if (!in || in->struct_size != sizeof(b200bpe_logits)) return refused("logits: struct_size is not that of b200bpe_logits");
     if (in->dtype > B200BPE_BF16) return refused("logits: unknown dtype");
     if (in->n_rows >= 1u << 27) return refused("logits: more than 2^27 - 1 rows");
     if (in->n_rows == 0) return B200BPE_OK;
+    if (!words(in->history, in->lengths, in->prompt_lengths, in->repetition, in->presence, in->frequency, in->bias_tokens, in->biases, in->mask, in->mask_rows))
+        return refused("logits: a misaligned pointer");
     const uint64_t size = in->dtype == B200BPE_F32 ? 4 : 2;
     if (!in->logits || reinterpret_cast<uint64_t>(in->logits) % size) return refused("logits: null or misaligned pointer");
     if (in->history) {
@@ -1513,6 +1519,7 @@ b200bpe_status b200bpe_sampler_sample(b200bpe_sampler* h, const b200bpe_logits* 
     const uint32_t vocab = h->s.vocab;
     if (in->n_rows == 0) return B200BPE_OK;
     if (!how->tokens_out) return refused("choice: null tokens_out");
+    if (!words(how->uniform, how->temperature, how->top_k, how->top_p, how->min_p, how->tokens_out, how->logprobs_out)) return refused("choice: a misaligned pointer");
     const OnDevice on(h->s.ctx->device);
     B2_CUDA(on.error);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

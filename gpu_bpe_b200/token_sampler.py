@@ -2,7 +2,7 @@
 
 No counterpart in the reference, whose tokens end in decode.  Inputs and outputs are torch tensors on the engine's GPU; the
 work is enqueued on torch's current stream and nothing is waited for, so calls can be captured into CUDA graphs.
-Token ids are int32 (or uint32), as encodeBatchDevice leaves them; -1 stands for no token.
+Token ids are int32 (or uint32), as encodeBatchDevice leaves them; -1 stands for no token.  Results carry no gradients.
 """
 from __future__ import annotations
 

@@ -276,7 +276,7 @@ void b200bpe_decoder_destroy(b200bpe_decoder*);
  * decode) ──
  * All pointers are device pointers on the context's GPU.  The calls only enqueue: `stream` is the caller's cudaStream_t (NULL is CUDA's default
  * stream), nothing is allocated, copied or waited for, and a handle holds no memory that a call writes; so calls can be captured into graphs, and
- * any number of threads, streams and graphs can use one handle at a time.  Inputs are only read, and have to stay as they are until the work is
+ * any number of threads, streams and graphs can use one handle at a time; it has to stay until their work is done.  Inputs are only read, and have to stay as they are until the work is
  * done; outputs must not overlap inputs, but for logits_out, which may be the logits themselves.  What a pointer's data says is taken as it
  * is: nothing in it makes a call fail or read out of range. */
 enum { B200BPE_F32 = 0, B200BPE_F16 = 1, B200BPE_BF16 = 2 };
@@ -293,7 +293,7 @@ enum { B200BPE_F32 = 0, B200BPE_F16 = 1, B200BPE_BF16 = 2 };
 typedef struct {
     uint32_t struct_size;           /* sizeof(b200bpe_logits); zero-initialise */
     uint32_t dtype;                 /* B200BPE_F32, _F16 or _BF16 */
-    uint32_t n_rows;
+    uint32_t n_rows;                /* fewer than 2^27 */
     uint32_t n_bias;                /* places of a row's list, at most 1,024 */
     const void* logits;             /* n_rows x at least the vocabulary's size; columns behind it are not looked at */
     uint64_t row_stride;            /* elements from a row to the next (the same for all strides: elements of their arrays) */

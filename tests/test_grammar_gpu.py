@@ -207,6 +207,8 @@ def test_c_entry_points(engine, torch):
     assert bad(L.b200bpe_grammar_mask(g._h, None, 1, t.data_ptr(), 1, None)) and bad(L.b200bpe_grammar_mask(g._h, t.data_ptr(), 1, None, 1, None))
     assert bad(L.b200bpe_grammar_mask(g._h, t.data_ptr(), 2, t.data_ptr(), 0, None)) and bad(L.b200bpe_grammar_mask(g._h, t.data_ptr(), 1 << 28, t.data_ptr(), 1, None))
     assert bad(L.b200bpe_grammar_advance(g._h, t.data_ptr(), t.data_ptr(), 1, t.data_ptr(), t.data_ptr(), 1, 1, None, None, None))
+    assert bad(L.b200bpe_grammar_mask(g._h, t.data_ptr() + 2, 1, t.data_ptr(), 1, None)) and bad(L.b200bpe_grammar_mask(g._h, t.data_ptr(), 1, t.data_ptr() + 1, 1, None))
+    assert bad(L.b200bpe_grammar_advance(g._h, t.data_ptr(), t.data_ptr() + 2, 1, t.data_ptr(), None, 0, 0, None, None, None))
     assert L.b200bpe_grammar_mask(g._h, None, 0, None, 0, None) == 0
     g.destroy()
 

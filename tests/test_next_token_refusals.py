@@ -183,6 +183,9 @@ def test_c_entry_points():
     both("null list", n_bias=2, biases=4096)
     both("mask_rows without", mask_rows=4096)
     both("fewer rows of the mask", mask=4096)
+    for field in ("history", "repetition", "biases", "mask", "mask_rows", "lengths"):
+        both("misaligned", **{field: 4098})
+    c.tokens_out = c.logprobs_out = 4096
     both("null handle")
     off, table = np.array([0, 1, 3], np.uint64), np.zeros((2, 256), np.uint32)
     ends, text = np.zeros(2, np.uint8), np.zeros(3, np.uint8)
