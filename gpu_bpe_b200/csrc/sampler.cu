@@ -422,6 +422,20 @@ constexpr uint32_t SM_QUICK_P0 = 64, SM_QUICK_P1 = 256;    // where so few weigh
 // that is a share u of a sum S has its part of the same errors: a running sum next to it is off from it by (1 - u) times what it is off itself, E(u S), less
 // u times what the rest is off, E((1 - u) S).  Where a running sum that decides lies within that of the border, the row's sums are made again of
 // weights in 64 bits.
+// 2^(i / 64), to the nearest.
+__device__ const double TWO_TO_64THS[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0, 0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0,
+    0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0, 0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0, 0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0,
+    0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0, 0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0, 0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0,
+    0x1.6247eb03a5585p+0, 0x1.6623882552225p+0, 0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0, 0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0,
+    0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0, 0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0, 0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0,
+    0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0, 0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
+
 struct Weights {
     float m, c, n;              // the largest x, log2 e / temperature, the exponent that all quick weights are relative to
     double steps;               // 64 log2 e / temperature
@@ -1102,6 +1116,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     const T* row = static_cast<const T*>(in.logits) + (uint64_t)sl.row * in.row_stride + sl.lo;
     uint4 ahead[SM_AHEAD];
     first_loads(row, sl, ahead);
+    const double power_64 = TWO_TO_64THS[threadIdx.x % 64];
     const Settings set(how, sl.row, vocab);
     const bool by_k = set.top_k != 0u, by_p = set.top_p < 1.0f, quick_k = by_k && set.top_k <= SM_QUICK_K;
     const bool quick_p = !by_k && by_p && set.top_p > 0.0f;
@@ -1127,7 +1142,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         if (t.lane == 0) { s.m_warp[t.warp] = m; s.n_warp[t.warp] = n; s.part_warp[0][t.warp] = sum; }
         if (threadIdx.x == 0) { s.at = 0xFFFFFFFFu; s.quick_candidates = 0u; }
         if (threadIdx.x < 4) s.cut[threadIdx.x] = -INFINITY;
-        if (threadIdx.x < 64 && !set.greedy) s.table[threadIdx.x] = exp2((double)threadIdx.x / 64);
+        if (threadIdx.x < 64) s.table[threadIdx.x] = power_64;
         if (quick_k || quick_p) s.keys[threadIdx.x] = key_of(stats.m);
         else if (by_k)
             for (uint32_t i = threadIdx.x; i < SM_BINS; i += SM_THREADS) s.bins[i] = 0u;
@@ -1199,13 +1214,27 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         return;
     }
     if (set.greedy && (t.rank != 0 || t.warp != 0)) return;
+    auto falls = [&](double part) {          // where the draw falls; a lane's part: that of a CTA
+        Draw d;
+        const double stay = warp_sum(part);
+        d.target = (double)set.uniform * stay;
+        d.near = how_near(vocab, stay, set.uniform, false);
+        d.owner = t.first_above<SM_MAX_CLUSTER>(part, 0.0, d.target, &d.base);
+        return d;
+    };
+    const bool limits = by_k || by_p || set.min_p > 0.0f;
     // What all warps need to know of the row; one works it out.
     if (t.warp == 0) {
         Row r;
         const Weights w{m, stats.c, n, 0.0, nullptr};
         r.unit = w.to_largest();
-        r.quick_all = warp_sum(t.lane < t.C ? s.best[t.lane].sum * Stats::power(s.best[t.lane].n - n) : 0.0);
+        const double part = t.lane < t.C ? s.best[t.lane].sum * Stats::power(s.best[t.lane].n - n) : 0.0;
+        r.quick_all = warp_sum(part);
         r.all = r.quick_all * r.unit;
+        if (!set.greedy && !limits) {
+            const Draw d = falls(part * r.unit);
+            if (t.lane == 0) s.draw = d;
+        }
         r.steps = set.greedy ? 0.0 : 64 * 1.4426950408889634 / set.warm;
         // A value that all of the top_k, or all that top_p keeps, are not below, if there is such a one.
         r.from = -INFINITY;
@@ -1347,24 +1376,18 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         }
         return t.rank == draw.owner;
     };
-    auto falls = [&](double part) {          // a lane's part: that of a CTA
-        Draw d;
-        const double stay = warp_sum(part);
-        d.target = (double)set.uniform * stay;
-        d.near = how_near(vocab, stay, set.uniform, false);
-        d.owner = t.first_above<SM_MAX_CLUSTER>(part, 0.0, d.target, &d.base);
-        return d;
-    };
     if (draw.owner != 0xFFFFFFFFu) {
         if (t.rank == draw.owner) {
             const double mass = warp_sum(kept_mass<false>(sl, t.warp, w, kept));
             if (t.lane == 0) s.warp_mass[t.warp] = mass;
             __syncthreads();
         }
-    } else if (!by_k && !by_p && set.min_p == 0.0f) {
-        draw = falls(t.lane < t.C ? s.best[t.lane].sum * Stats::power(s.best[t.lane].n - n) * unit : 0.0);
-        if (threadIdx.x < SM_WARPS) s.warp_mass[threadIdx.x] = s.part_warp[0][threadIdx.x] * Stats::power(s.n_warp[threadIdx.x] - n) * unit;
-        __syncthreads();
+    } else if (!limits) {
+        draw = s.draw;
+        if (t.rank == draw.owner) {
+            if (threadIdx.x < SM_WARPS) s.warp_mass[threadIdx.x] = s.part_warp[0][threadIdx.x] * Stats::power(s.n_warp[threadIdx.x] - n) * unit;
+            __syncthreads();
+        }
     } else {
         double mass = kept_mass<false>(sl, t.warp, w, kept), none = 0;
         t.total(mass, none);
