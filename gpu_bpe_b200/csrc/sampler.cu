@@ -1288,14 +1288,26 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     if (quick) {
         from = fmaxf(from, -3.402823466e38f);            // (-infinity is never chosen)
         Shared* lead = t.peer(0);
-        each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
-            const float v[4] = {x.x, x.y, x.z, x.w};
-            if (!__any_sync(0xFFFFFFFFu, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= from)) return;
-            uint32_t in = 0;
+        // (most groups of 512 places have none)
+        const Span span(sl.padded, t.warp);
+        for (uint32_t p0 = span.lo + t.lane * 4; p0 < span.hi + t.lane * 4; p0 += 512) {
+            float4 x[4];
+            float top = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < 4; k++) in |= (uint32_t)(v[k] >= from) << k;
-            gather(t, &s.quick_candidates, s.list, v, in, p + shift);
-        });
+            for (int j = 0; j < 4; j++) {
+                x[j] = p0 + j * 128 < span.hi ? *reinterpret_cast<const float4*>(buf + p0 + j * 128) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                top = fmaxf(top, fmaxf(fmaxf(x[j].x, x[j].y), fmaxf(x[j].z, x[j].w)));
+            }
+            if (!__any_sync(0xFFFFFFFFu, top >= from)) continue;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float v[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+                uint32_t in = 0;
+#pragma unroll
+                for (int k = 0; k < 4; k++) in |= (uint32_t)(v[k] >= from) << k;
+                gather(t, &s.quick_candidates, s.list, v, in, p0 + j * 128 + shift);
+            }
+        }
         hand_over(t, &Shared::quick_candidates);
         t.sync();
         const uint32_t so_many = lead->quick_candidates;
