@@ -1390,8 +1390,19 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
     };
     if (draw.owner != 0xFFFFFFFFu) {
         if (t.rank == draw.owner) {
-            const double mass = warp_sum(kept_mass<false>(sl, t.warp, w, kept));
-            if (t.lane == 0) s.warp_mass[t.warp] = mass;
+            // Every warp's sum of what lies above the border's bins is there; of the candidates those that stay are added.  The CTA's own are still in its
+            // list, and the first CTA's has all of them, with their weights.
+            const Span span(sl.padded, t.warp);
+            double mass = 0;
+            for (uint32_t i = t.lane; i < s.candidates; i += 32) {
+                const unsigned long long e = s.list[i];
+                const uint32_t v = ~(uint32_t)(t.rank ? e : e >> 32), p = v - shift;
+                if (p < span.lo || p >= span.hi || v < sl.lo || v - sl.lo >= sl.len) continue;
+                if (t.rank == 0) mass += (double)__uint_as_float((uint32_t)e);
+                else if (const float x = value_of((uint32_t)(e >> 32)); kept.has(x, v)) mass += (double)w.quick(x) * unit;
+            }
+            mass = warp_sum(mass);
+            if (t.lane == 0) s.warp_mass[t.warp] += mass;
             __syncthreads();
         }
     } else if (!limits) {
