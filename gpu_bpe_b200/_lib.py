@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libb200bpe.so")
@@ -63,6 +64,10 @@ class Logits(C.Structure):
                 ("prompt_lengths", C.c_void_p), ("history_cap", C.c_uint32), ("n_mask_rows", C.c_uint32), ("repetition", C.c_void_p),
                 ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias_tokens", C.c_void_p), ("biases", C.c_void_p),
                 ("bias_stride", C.c_uint64), ("mask", C.c_void_p), ("mask_stride", C.c_uint64), ("mask_rows", C.c_void_p)]
+
+
+# The same as bytes, for calls that are made once a token: packing takes half a microsecond, a Structure two.
+PACKED_LOGITS, PACKED_CHOICE = struct.Struct("@IIIIPQPQPPIIPPPPPQPQP"), struct.Struct("@IIPPPPPPP")
 
 
 class Choice(C.Structure):
@@ -123,8 +128,8 @@ SIGNATURES = {
     "b200bpe_decoder_read": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64]),
     "b200bpe_decoder_destroy": (None, [C.c_void_p]),
     "b200bpe_sampler_create": (C.c_int32, [C.c_void_p, C.c_uint32, C.POINTER(C.c_void_p)]),
-    "b200bpe_sampler_adjust": (C.c_int32, [C.c_void_p, C.POINTER(Logits), C.c_void_p, C.c_uint64, C.c_void_p]),
-    "b200bpe_sampler_sample": (C.c_int32, [C.c_void_p, C.POINTER(Logits), C.POINTER(Choice), C.c_void_p]),
+    "b200bpe_sampler_adjust": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "b200bpe_sampler_sample": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "b200bpe_sampler_destroy": (None, [C.c_void_p]),
     "b200bpe_grammar_create": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32,
                                            C.POINTER(C.c_void_p)]),

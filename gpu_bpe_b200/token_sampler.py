@@ -80,9 +80,9 @@ class TokenSampler:
         self._h = h
 
     def _row(self, keep, value, name, shape, kinds):
-        """Address of one value a row; None has none, a plain number stands for all rows."""
+        """Address of one value a row; None has none (0), a plain number stands for all rows."""
         if value is None:
-            return None
+            return 0
         index = self._engine.device_index
         if isinstance(value, (int, float)):
             import torch
@@ -99,7 +99,7 @@ class TokenSampler:
         rows = shape[0]
         if columns < self.vocabSize:
             raise ValueError(f"logits: {columns} columns, the vocabulary has {self.vocabSize} tokens")
-        p_history = p_lengths = p_prompt = p_rep = p_pres = p_freq = p_ids = p_biases = p_mask = p_which = None
+        p_history = p_lengths = p_prompt = p_rep = p_pres = p_freq = p_ids = p_biases = p_mask = p_which = 0
         history_stride = room = n_bias = bias_stride = mask_stride = mask_rows = 0
         if history is not None:
             if lengths is None:
@@ -111,7 +111,7 @@ class TokenSampler:
             p_pres = self._row(keep, presence, "presence", shape, FLOATS)
             p_freq = self._row(keep, frequency, "frequency", shape, FLOATS)
             if not room:
-                p_history = p_lengths = p_prompt = p_rep = p_pres = p_freq = None
+                p_history = p_lengths = p_prompt = p_rep = p_pres = p_freq = 0
         elif not (lengths is None and promptLengths is None and repetition is None and presence is None and frequency is None):
             raise ValueError("history: needed for lengths and penalties")
         if biasTokens is not None or biases is not None:
@@ -138,8 +138,8 @@ class TokenSampler:
                 raise ValueError(f"mask: {mask_rows} rows for {rows} rows of logits, and no maskRows")
         elif maskRows is not None:
             raise ValueError("maskRows: needs a mask")
-        return _lib.Logits(LOGITS_BYTES, LOGITS[logits.dtype], rows, n_bias, p_logits, row_stride, p_history, history_stride, p_lengths, p_prompt,
-                           room, mask_rows, p_rep, p_pres, p_freq, p_ids, p_biases, bias_stride, p_mask, mask_stride, p_which)
+        return rows, _lib.PACKED_LOGITS.pack(LOGITS_BYTES, LOGITS[logits.dtype], rows, n_bias, p_logits, row_stride, p_history, history_stride, p_lengths,
+                                             p_prompt, room, mask_rows, p_rep, p_pres, p_freq, p_ids, p_biases, bias_stride, p_mask, mask_stride, p_which)
 
     def adjustLogits(self, logits, out=None, history=None, lengths=None, promptLengths=None, repetition=None, presence=None, frequency=None,
                      biasTokens=None, biases=None, mask=None, maskRows=None):
@@ -151,17 +151,17 @@ class TokenSampler:
         biasTokens, biases [rows, n]: ids (-1: unused place) and what is added.  mask [rows, words]: bit v & 31 of word v >> 5 allows token v, as
         TokenGrammar.allowedTokens makes them; with maskRows, row maskRows[r] of it is row r's, and none allows anything."""
         keep = []
-        p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
+        rows, p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
         if out is None:
-            out = logits.new_empty((logits.size(0), self.vocabSize))
-        address, stride, columns = table_of(out, "out", self._engine.device_index, LOGITS, p.n_rows)
+            out = logits.new_empty((rows, self.vocabSize))
+        address, stride, columns = table_of(out, "out", self._engine.device_index, LOGITS, rows)
         if out.dtype != logits.dtype:
             raise ValueError(f"out: a tensor of {logits.dtype} is needed")
         if columns < self.vocabSize:
             raise ValueError(f"out: {columns} columns, the vocabulary has {self.vocabSize} tokens")
-        if stride < self.vocabSize and p.n_rows > 1:
+        if stride < self.vocabSize and rows > 1:
             raise ValueError("out: rows overlap")
-        status = _lib.lib().b200bpe_sampler_adjust(self._h, C.byref(p), address, stride, raw_stream(self._engine.device_index))
+        status = _lib.lib().b200bpe_sampler_adjust(self._h, p, address, stride, raw_stream(self._engine.device_index))
         if status:
             _lib.check(status, "b200bpe_sampler_adjust")
         return out
@@ -176,9 +176,9 @@ class TokenSampler:
         2^-16: the largest.  Each is one number a row, or one for all.  logprobs are under the weights of all allowed tokens (at temperature 1
         where the largest is taken).  A row without an allowed token gives -1 and -inf; a NaN is never chosen."""
         keep = []
-        p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
+        rows, p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
         shape = logits.shape[:1]
-        p_uniform = p_warm = p_k = p_p = p_m = None
+        p_uniform = p_warm = p_k = p_p = p_m = 0
         if uniform is not None:
             p_uniform = row_of(uniform, "uniform", self._engine.device_index, FLOATS, shape)
             p_warm = self._row(keep, temperature, "temperature", shape, FLOATS)
@@ -188,9 +188,9 @@ class TokenSampler:
         elif not (temperature is None and topK is None and topP is None and minP is None):
             raise ValueError("uniform: needed to draw")
         import torch
-        tokens, logprobs = logits.new_empty(p.n_rows, dtype=torch.int32), logits.new_empty(p.n_rows, dtype=torch.float32)
-        c = _lib.Choice(CHOICE_BYTES, 0, p_uniform, p_warm, p_k, p_p, p_m, tokens.data_ptr(), logprobs.data_ptr())
-        status = _lib.lib().b200bpe_sampler_sample(self._h, C.byref(p), C.byref(c), raw_stream(self._engine.device_index))
+        tokens, logprobs = logits.new_empty(rows, dtype=torch.int32), logits.new_empty(rows, dtype=torch.float32)
+        c = _lib.PACKED_CHOICE.pack(CHOICE_BYTES, 0, p_uniform, p_warm, p_k, p_p, p_m, tokens.data_ptr(), logprobs.data_ptr())
+        status = _lib.lib().b200bpe_sampler_sample(self._h, p, c, raw_stream(self._engine.device_index))
         if status:
             _lib.check(status, "b200bpe_sampler_sample")
         return tokens, logprobs

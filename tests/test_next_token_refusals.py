@@ -219,3 +219,12 @@ def test_the_model_by_hand():
     table, ends = model.literals([b"ab", b"abc"])
     assert model.allowed([b"a", b"abc", b"b", b"", b"x", b"e"], table, ends, 5, 0).tolist() == [True, True, False, False, False, False]
     assert model.allowed([b"c", b"cc", b"e"], table, ends, 2, 2).tolist() == [True, False, True]
+
+
+def test_packed_structures():
+    """What the calls pack is what the header's structures are."""
+    for packed, of in ((_lib.PACKED_LOGITS, _lib.Logits), (_lib.PACKED_CHOICE, _lib.Choice)):
+        assert packed.size == C.sizeof(of)
+        values = list(range(1, len(of._fields_) + 1))
+        got = of.from_buffer_copy(packed.pack(*values))
+        assert [getattr(got, name) for name, _ in of._fields_] == values
