@@ -257,20 +257,20 @@ __device__ __forceinline__ void each_adjusted(const T* row, const Slice& s, uint
             if (any_special) {
                 constexpr uint32_t ALL = (1u << N) - 1u;
                 if (const uint32_t any = special.any[p >> 5] >> (p & 31u) & ALL) {
-                    const uint32_t seen = special.seen[p >> 5] >> (p & 31u);
-                    if (seen & ALL) {
+                    const uint32_t seen = special.seen[p >> 5] >> (p & 31u) & ALL;
+                    // (what is seen has its x in the buffer; the others are masked)
+                    if (seen) {
 #pragma unroll
                         for (uint32_t k = 0; k < N; k += 4) {
                             const float4 x = *reinterpret_cast<const float4*>(s.buf + p + k);
-                            v[k] = seen >> k & 1u ? x.x : v[k];
-                            v[k + 1] = seen >> (k + 1) & 1u ? x.y : v[k + 1];
-                            v[k + 2] = seen >> (k + 2) & 1u ? x.z : v[k + 2];
-                            v[k + 3] = seen >> (k + 3) & 1u ? x.w : v[k + 3];
-                        }
-                    }
-                    const uint32_t deny = any & ~seen;
+                            const float y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (uint32_t k = 0; k < N; k++) v[k] = deny >> k & 1u ? -INFINITY : v[k];
+                            for (uint32_t i = 0; i < 4; i++) v[k + i] = any & (1u << (k + i)) ? seen & (1u << (k + i)) ? y[i] : -INFINITY : v[k + i];
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t k = 0; k < N; k++) v[k] = any & (1u << k) ? -INFINITY : v[k];
+                    }
                 }
             }
             to(p, v);
