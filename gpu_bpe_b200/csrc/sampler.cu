@@ -1097,12 +1097,12 @@ __device__ bool choose_from_list(Team& t, const Weights& w, const Settings& set,
 //   top_k of up to SM_QUICK_K, and a top_p that few tokens make up: the candidates go to the first CTA, which sorts them and does the rest in 64 bits;
 //   otherwise: bins (counts or weights) of the whole row say between which two values the border lies, the candidates between them are sorted, and the
 //   draw is made over what is above; should ties leave more than SM_CANDIDATES, a bisection of the values takes over.
-// 256 rows of 131,072 in 16 bits (67 MB: 10.2 us at the memory's rate), no penalties: 40 us for the largest x, 77 for a draw, 82 with top_k 50, 114 with top_k 400,
-// 231 with a top_p of 0.9 that keeps thousands of tokens and 113 with one that keeps few; histories of 1,500 tokens add some 23.  One row of 32,256:
+// 256 rows of 131,072 in 16 bits (67 MB: 10.2 us at the memory's rate), no penalties: 40 us for the largest x, 75 for a draw, 78 with top_k 50, 112 with top_k 400,
+// 216 with a top_p of 0.9 that keeps thousands of tokens and 109 with one that keeps few; histories of 1,500 tokens add some 23.  One row of 32,256:
 // 5 us, 8, 14, 20, 26 and 16.  Neither memory nor arithmetic bounds it but the length of a row's way through the cluster's barriers: loading
 // takes 9,000 cycles of a CTA (24 warps to an SM; exponentials alone 3,000), the first exchange 4,500, a draw 7,000, bins and border some 40,000.  An SM has three
 // CTAs, by registers and shared memory.  Slices of 16,384 tokens are the largest of which three fit; smaller ones (clusters of 12 or 16, four CTAs to an
-// SM) gain nothing, since what a warp does once for a row, some 600 instructions, is half of all it does at that size (168 us against 137 for a mixed batch).
+// SM) gain nothing, since what a warp does once for a row, some 600 instructions, is half of all it does at that size (168 us against 137 for a mixed batch, when both were measured).
 template <class T>
 __global__ void __launch_bounds__(SM_THREADS, 3)
 k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200bpe_choice how, uint32_t vocab) {
