@@ -940,7 +940,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                         if (k < each) s.list[i] = s.list[i] << 32 | __float_as_uint(i <= s.place ? (float)v[k] : 0.0f);
                     }
                     __syncthreads();
-                                        for (uint32_t c = t.warp; c < t.C; c += SM_WARPS) {
+                    for (uint32_t c = t.warp; c < t.C; c += SM_WARPS) {
                         double part = 0;
                         for (uint32_t i = t.lane; i < n; i += 32) {
                             const uint32_t token = ~(uint32_t)(s.list[i] >> 32);
