@@ -341,7 +341,8 @@ k_adjust(const __grid_constant__ b200bpe_logits in, uint32_t vocab, uint32_t who
 // A thread's largest x, the place of the first vector that has it, and the sum of 2^(x c - n) over its x, n being a whole number next to the largest
 // x c: sums with different n are brought to one another by powers of two, without rounding.
 struct Stats {
-    static constexpr float FAR = 8589934592.0f;      // 2^33: where x c lies further out, neighbouring floats are 512 powers of two apart
+    // 2^25: up to there the whole number is within 1 of x c (half of a step between floats; further out a weight of the largest x itself could be 2^256).
+    static constexpr float FAR = 33554432.0f;
     float c, m = -INFINITY, n = -FAR;
     uint32_t at = 0;
     double sum = 0;
@@ -1197,7 +1198,8 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         m = value_of(__reduce_max_sync(0xFFFFFFFFu, t.lane < t.C ? key_of(s.best[t.lane].m) : LOWEST_KEY));
         n = stats.base(m);
         if (again || m == -INFINITY || fabsf(m) * stats.c < Stats::FAR) break;
-        // So far out that only differences from m mean something.
+        // So far out that x c has no whole number in 32 bits next to it: with differences from m.  They are exact from m / 2 to 2 m, and what lies
+        // further off weighs nothing.
         for (uint32_t p = threadIdx.x; p < sl.padded; p += SM_THREADS) buf[p] = buf[p] == m ? 0.0f : m == INFINITY ? -INFINITY : buf[p] - m;
         __syncthreads();
         Stats near;

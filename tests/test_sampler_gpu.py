@@ -253,6 +253,32 @@ def test_odd_values_in_a_choice(engine, torch):
     s.destroy()
 
 
+@pytest.mark.parametrize("low", [-1e9, -2e9, -5e9, -65504.0, -3e4, -1e38])
+def test_low_values_and_temperatures(engine, torch, low):
+    """Tokens put far below the others, rows that lie far out as a whole, at temperatures that make x / temperature large."""
+    vocab, rows = 6000, 12
+    rng = np.random.default_rng(6)
+    s = TokenSampler(engine, vocab)
+    _, values = _logits(rng, rows, vocab, "float32", torch)
+    values[:3][rng.random((3, vocab)) < 0.5] = low
+    values[3:6, 40:5900] = low
+    values[6] += 400
+    values[7] += 3e4
+    values[8] += 1e8
+    values[9] -= 2e9
+    values[10, :] = low
+    values[11, :] = low
+    values[11, 17] = low / 2
+    t = _cuda(torch, values)
+    u = rng.random(rows).astype(np.float32)
+    _compare(values, *_sample(torch, s, t), vocab)
+    for warm in (1.0, 0.9, 0.7, 0.6, 0.4, 0.3, 0.2, 1e-3, 3e-5, 2.0 ** -16):
+        for st in ({}, {"k": np.full(rows, 50, np.int32)}, {"k": np.full(rows, 3000, np.int32)}, {"p": np.full(rows, 0.9, np.float32)}, {"m": np.full(rows, 0.1, np.float32)}):
+            st = dict(st, t=np.full(rows, warm, np.float32))
+            _compare(values, *_sample(torch, s, t, u, st), vocab, u, **st)
+    s.destroy()
+
+
 def test_masks_shared_by_rows(engine, torch):
     vocab, rows = 2100, 7
     rng = np.random.default_rng(5)
