@@ -416,13 +416,19 @@ constexpr uint32_t SM_QUICK_P0 = 64, SM_QUICK_P1 = 256;    // where so few weigh
 // Which token is chosen depends on sums of weights: on the first running sum that is above a border.  Sums are made of weights in 32 bits,
 // w = 2^(x c - n) with c = log2 e / temperature, and added in 64 bits.  Against the exact weights, up to a factor that all have in common, the
 // exponent is off by the roundings of log2 e, c and the product's difference, together 2.5 * 2^-24 (m - x) c + 2^-24, the exponential by 2^-22 of itself, and up to
-// eight weights are added in 32 bits first, three roundings: a sum is off by at most
-//     E = sum w * 2^-24 * (10 + 2.5 ln 2 (m - x) c),
-// with two for the factor that brings such sums to the unit of the others, where that matters.
-// The mean of (m - x) c under some tokens' weights is their entropy less log2 r, r = sum w / the row's largest w, so at most log2(tokens / r).  A border
-// that is a share u of a sum S has its part of the same errors: a running sum next to it is off from it by (1 - u) times what it is off itself, E(u S), less
-// u times what the rest is off, E((1 - u) S).  Where a running sum that decides lies within that of the border, the row's sums are made again of
-// weights in 64 bits.
+// eight weights are added in 32 bits first, three roundings.  The factor that brings such sums to the unit of exact ones is an exp2f, off by 2 of its last places,
+// 2^-22, and the rounding of its argument.  So a sum is off by at most
+//     E = sum w * 2^-24 * (13 + 2.5 ln 2 (m - x) c).
+// The mean of (m - x) c under some tokens' weights is their entropy less log2 r, r = sum w / the row's largest w, so at most log2(tokens / r).
+//
+// A running sum F is compared with a border that is a share u of the whole S = F + R.
+//   Where S was made of the same sums as F, what F is off is also in S: F - u S is off by (1 - u) times what F is off, less u times what R is.  At the
+//   border F is u S, so that this is at most (1 - u) E(u S) + u E((1 - u) S).
+//   Where a part G of F was added in another order than in S (the places of one warp's part, in find_place), its errors are not the same: they are at
+//   most E(G) and u E(G) where (1 - u) E(G) was counted, so 2 u E(G) more, and G's own roundings.
+//   Where F is exact, u E(S); where the border is, E(u S).
+// Sums in 64 bits are off by some steps of 2^-53 besides, and weights below 2^-126 count for nothing in 32 bits: 2^-44 S has room for both.  Where a
+// running sum that decides lies within all that of the border, the row's sums are made again of weights in 64 bits.
 // 2^(i / 64), to the nearest.
 __device__ const double TWO_TO_64THS[64] = {
     0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0, 0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0,
@@ -455,11 +461,17 @@ struct Weights {
     __device__ __forceinline__ double to_largest() const { return (double)exp2f((float)power_of_largest()); }        // quick's unit in exact's
 };
 
-// How far a running sum may be off from a share of the sum, both of quick weights; or, `exact`, from a border that is exact.
-__device__ __forceinline__ double how_near(uint32_t vocab, double sum, double share, bool exact) {
-    auto off = [&](float r) { return r > 0.0f ? r * (10.0f + 1.75f * (1.0f + log2f((float)vocab / r))) : 0.0f; };
-    const float a = off((float)(share * sum)), b = off((float)((1.0 - share) * sum));
-    return (double)(exact ? a : (float)(1.0 - share) * a + (float)share * b) * (1.01 / 16777216.0);
+// E of quick weights whose sum is r, in parts of 2^-24.
+__device__ __forceinline__ float off_by(uint32_t vocab, float r) { return r > 0.0f ? r * (13.0f + 1.75f * (1.0f + log2f((float)vocab / r))) : 0.0f; }
+constexpr double SM_OFF = 1.01 / 16777216.0;         // (what `off_by` is off itself, and the difference between F and u S)
+// How far a running sum may be off from its border, a share of `sum`.
+enum class Border { OF_ITS_SUM, EXACT, OF_EXACT_SUMS };        // quick sums, the one made of the other; quick sums, an exact border; exact sums, a share of a quick one
+__device__ __forceinline__ double how_near(uint32_t vocab, double sum, double share, Border border) {
+    double off;
+    if (border == Border::OF_ITS_SUM) off = (1.0 - share) * off_by(vocab, (float)(share * sum)) + share * off_by(vocab, (float)((1.0 - share) * sum));
+    else if (border == Border::EXACT) off = off_by(vocab, (float)(share * sum));
+    else off = share * off_by(vocab, (float)sum);
+    return off * SM_OFF + sum * 0x1p-44;
 }
 
 // What of the row is kept: x with a larger key, and those with the key in front of token `end`.
@@ -606,14 +618,16 @@ __device__ __forceinline__ double kept_mass(const Slice& sl, int warp, const Wei
 }
 
 // The first place of the slice at which base plus the running sum of f(place, x) is above target; if there is none, the last with f above 0.  Every
-// warp's sum of f is in s.warp_mass.  *near: whether a sum that decided was within `margin` of target (or the sums of parts and of places round apart).
+// warp's sum of f is in s.warp_mass.  *near: whether a sum that decided was within `margin` of target (or the sums of parts and of places round apart);
+// for quick weights, whose target is a `share` of all of them, and whose sums up to a warp's part are `margin` off, what that part adds comes to it.
 // Called by all threads of one CTA: first the part of a warp, then a step of 128 places of it, then a place.  f gives V.
 template <class V, class F>
-__device__ uint32_t find_place(Team& t, const Slice& sl, double base, double target, double margin, bool* near, F f) {
+__device__ uint32_t find_place(Team& t, const Slice& sl, double base, double target, double margin, double share, uint32_t vocab, bool* near, F f) {
     static_assert(SM_MAX_SLICE + 8 <= SM_WARPS * 32 * 128, "more than 32 steps in a warp's part");
     constexpr int EACH = 32 / SM_WARPS;
     Shared& s = t.s;
     const Span span(sl.padded, t.first_above<SM_WARPS>(t.lane < SM_WARPS ? s.warp_mass[t.lane] : 0.0, base, target, &base));
+    const double part = base;        // what is in front of the warp's part
     // A warp has EACH of the steps, a lane four neighbouring places of each.
     V v[EACH][4], run[EACH];
 #pragma unroll
@@ -636,7 +650,11 @@ __device__ uint32_t find_place(Team& t, const Slice& sl, double base, double tar
     const int step = t.first_above(mass, base, target, &base);
     if (step % SM_WARPS == t.warp) {
         const double whole = __shfl_sync(0xFFFFFFFFu, mass, step);
-        if (sizeof(V) == 4) margin += whole * (10.0 / 16777216);          // (within a step: a product, the sums of four, five steps of a scan, two differences)
+        if (sizeof(V) == 4) {
+            // (the roundings of the part's own sums: of the unit, a product, two sums of four, five steps of a scan, a difference)
+            const double front = base + whole - part;
+            margin += (10.0 * front + 2.0 * share * off_by(vocab, (float)front)) * SM_OFF;
+        }
         uint32_t hit = 0, last = 0;
         bool edge = false;
 #pragma unroll
@@ -882,7 +900,10 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     t.sync();
     // sums of what is above the border's bins; what lies in them goes to the first CTA
     const float high = bins.end_of(s.border[0], false), low = bins.end_of(max(s.border[0], s.border[1]), true);
-    double above = 0, count = 0;
+    // A border that is a share of all: `rest`, what lies below the border's bins, makes the whole of the same sums as what lies above.  (9 us of 225 for a
+    // top_p of 0.9 and 256 rows of 131,072; against the whole as it was loaded, a border would be four times as far from certain.)
+    const double unit = MASS ? w.to_largest() : 1.0;
+    double above = 0, rest = 0;
     each_four(sl, t.warp, [&](uint32_t p, const float4& x) {
         const float v[4] = {x.x, x.y, x.z, x.w};
         uint32_t in = 0;
@@ -894,11 +915,18 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
             for (int k = 0; k < 4; k++) e[k] = v[k] > high ? MASS ? w.quick(v[k]) : 1.0f : 0.0f;
             above += (double)((e[0] + e[1]) + (e[2] + e[3]));
         }
+        if (MASS && share >= 0) {
+            float e[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) e[k] = v[k] < low ? w.quick(v[k]) : 0.0f;
+            rest += (double)((e[0] + e[1]) + (e[2] + e[3]));
+        }
         gather(t, &s.candidates, s.list, v, in, p + shift);      // (the list lies where the bins were)
     });
     hand_over(t, &Shared::candidates);
-    if (MASS) above *= w.to_largest();
-    t.total(above, count);
+    above *= unit;
+    rest *= unit;
+    t.total(above, rest);
     const uint32_t n = t.peer(0)->candidates;
     if (n <= SM_CANDIDATES) {
         uint32_t each = 1;
@@ -915,7 +943,8 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                     mine += v[k];
                 }
                 if (threadIdx.x == 0) { s.flag = 0u; s.place = n ? n - 1 : 0u; }
-                double ignored, sum = above + t.before(mine, &ignored);
+                double of_list, sum = above + t.before(mine, &of_list);
+                if (MASS && share >= 0 && turn == 0) target = share * (above + of_list + rest);
 #pragma unroll
                 for (uint32_t k = 0; k < SM_EACH; k++) {
                     const double next = sum + v[k];
@@ -933,12 +962,13 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                 const uint32_t near_some = s.flag;
                 Draw draw{0xFFFFFFFFu, 0.0, 0.0, 0.0};
                 if (MASS && set && near_some == 0u && turn == 0 && set->min_key(w.m) <= kept.key) {
-                    // Nothing else takes tokens away: the kept ones' weights by CTA are known, and so is where the draw falls.
+                    // Nothing else takes tokens away: the kept ones' weights by CTA are known, and so is where the draw falls.  (Quick weights, so that
+                    // the sums of CTAs and of their warps are the same ones.)
                     __syncthreads();
 #pragma unroll
                     for (uint32_t k = 0; k < SM_EACH; k++) {
                         const uint32_t i = threadIdx.x * each + k;
-                        if (k < each) s.list[i] = s.list[i] << 32 | __float_as_uint(i <= s.place ? (float)v[k] : 0.0f);
+                        if (k < each) s.list[i] = s.list[i] << 32 | __float_as_uint(i <= s.place ? w.quick(value_of((uint32_t)(s.list[i] >> 32))) : 0.0f);
                     }
                     __syncthreads();
                     for (uint32_t c = t.warp; c < t.C; c += SM_WARPS) {
@@ -948,13 +978,13 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
                             if (token - c * whole < whole) part += (double)__uint_as_float((uint32_t)s.list[i]);
                         }
                         part = warp_sum(part);
-                        if (t.lane == 0) s.step_mass[c] = part + t.part(0, c);
+                        if (t.lane == 0) s.step_mass[c] = part * unit + t.part(0, c);
                     }
                     __syncthreads();
                     const double part = t.lane < t.C ? s.step_mass[t.lane] : 0.0;
                     const double stay = warp_sum(part);
                     draw.target = (double)set->uniform * stay;
-                    draw.near = how_near(vocab, stay, set->uniform, false);
+                    draw.near = how_near(vocab, stay, set->uniform, Border::OF_ITS_SUM);
                     draw.owner = t.first_above<SM_MAX_CLUSTER>(part, 0.0, draw.target, &draw.base);
                 }
                 if (threadIdx.x < t.C) {
@@ -1023,7 +1053,7 @@ __device__ Kept border(Team& t, const Slice& sl, const Weights& w, const Bins& b
     const uint32_t owner = t.first_above<SM_MAX_CLUSTER>(t.lane < t.C ? t.part(0, t.lane) : 0.0, 0.0, ties - 0.5, &base);
     if (t.rank == owner) {
         bool near;
-        const uint32_t p = find_place<double>(t, sl, base, ties - 0.5, 0.0, &near, [&](uint32_t, float x) { return key_of(x) == least ? 1.0 : 0.0; });
+        const uint32_t p = find_place<double>(t, sl, base, ties - 0.5, 0.0, 0.0, vocab, &near, [&](uint32_t, float x) { return key_of(x) == least ? 1.0 : 0.0; });
         if (threadIdx.x < t.C) t.peer(threadIdx.x)->cut_at[1] = p + shift + 1u;
     }
     t.sync();
@@ -1098,9 +1128,9 @@ __device__ bool choose_from_list(Team& t, const Weights& w, const Settings& set,
 //   top_k of up to SM_QUICK_K, and a top_p that few tokens make up: the candidates go to the first CTA, which sorts them and does the rest in 64 bits;
 //   otherwise: bins (counts or weights) of the whole row say between which two values the border lies, the candidates between them are sorted, and the
 //   draw is made over what is above; should ties leave more than SM_CANDIDATES, a bisection of the values takes over.
-// 256 rows of 131,072 in 16 bits (67 MB: 10.2 us at the memory's rate), no penalties: 40 us for the largest x, 75 for a draw, 78 with top_k 50, 112 with top_k 400,
-// 216 with a top_p of 0.9 that keeps thousands of tokens and 109 with one that keeps few; histories of 1,500 tokens add some 23.  One row of 32,256:
-// 5 us, 8, 14, 20, 26 and 16.  Neither memory nor arithmetic bounds it but the length of a row's way through the cluster's barriers: loading
+// 256 rows of 131,072 in 16 bits (67 MB: 10.2 us at the memory's rate), no penalties: 40 us for the largest x, 78 for a draw, 77 with top_k 50, 111 with top_k 400,
+// 225 with a top_p of 0.9 that keeps thousands of tokens and 106 with one that keeps few; histories of 1,500 tokens add some 23.  One row of 32,256:
+// 5 us, 9, 13, 19, 26 and 14.  Neither memory nor arithmetic bounds it but the length of a row's way through the cluster's barriers: loading
 // takes 9,000 cycles of a CTA (24 warps to an SM; exponentials alone 3,000), the first exchange 4,500, a draw 7,000, bins and border some 40,000.  An SM has three
 // CTAs, by registers and shared memory.  Slices of 16,384 tokens are the largest of which three fit; smaller ones (clusters of 12 or 16, four CTAs to an
 // SM) gain nothing, since what a warp does once for a row, some 600 instructions, is half of all it does at that size (168 us against 137 for a mixed batch, when both were measured).
@@ -1220,7 +1250,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         Draw d;
         const double stay = warp_sum(part);
         d.target = (double)set.uniform * stay;
-        d.near = how_near(vocab, stay, set.uniform, false);
+        d.near = how_near(vocab, stay, set.uniform, Border::OF_ITS_SUM);
         d.owner = t.first_above<SM_MAX_CLUSTER>(part, 0.0, d.target, &d.base);
         return d;
     };
@@ -1327,7 +1357,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
             cluster.barrier_wait();
         } else if (so_many <= SM_CANDIDATES) {
             if (t.rank == 0) {
-                const bool done = choose_from_list(t, w, set, so_many, all, how_near(vocab, all, set.top_p, false), &x, &token);
+                const bool done = choose_from_list(t, w, set, so_many, all, how_near(vocab, all, set.top_p, Border::OF_EXACT_SUMS), &x, &token);
                 if (threadIdx.x == 0 && done) answer(token, x);
                 if (threadIdx.x < t.C) t.peer(threadIdx.x)->again = !done;
             }
@@ -1366,7 +1396,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
                 bins.put<true>(s.bins, x, end);
             });
             t.sync();
-            k = border<true>(t, sl, w, bins, (double)set.top_p * whole, by_k ? -1.0 : (double)set.top_p, how_near(vocab, whole, set.top_p, by_k),
+            k = border<true>(t, sl, w, bins, (double)set.top_p * whole, by_k ? -1.0 : (double)set.top_p, how_near(vocab, whole, set.top_p, by_k ? Border::EXACT : Border::OF_ITS_SUM),
                              by_k ? nullptr : &set, vocab, draw);
         } else {
             uint32_t token = 0xFFFFFFFFu;
@@ -1384,8 +1414,8 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         constexpr bool EXACT = decltype(exact)::value;
         if (t.rank == draw.owner) {
             bool near;
-            if (EXACT) *place = find_place<double>(t, sl, draw.base, draw.target, 0.0, &near, [&](uint32_t p, float x) { return kept.has(x, p + shift) ? w.exact(x) : 0.0; });
-            else *place = find_place<float>(t, sl, draw.base, draw.target, draw.near, &near, [&](uint32_t p, float x) { return kept.has(x, p + shift) ? w.quick(x) * (float)unit : 0.0f; });
+            if (EXACT) *place = find_place<double>(t, sl, draw.base, draw.target, 0.0, 0.0, vocab, &near, [&](uint32_t p, float x) { return kept.has(x, p + shift) ? w.exact(x) : 0.0; });
+            else *place = find_place<float>(t, sl, draw.base, draw.target, draw.near, set.uniform, vocab, &near, [&](uint32_t p, float x) { return kept.has(x, p + shift) ? w.quick(x) * (float)unit : 0.0f; });
             if (!EXACT && threadIdx.x < t.C) t.peer(threadIdx.x)->cut_at[0] = near;
         }
         return t.rank == draw.owner;
@@ -1400,7 +1430,7 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
                 const unsigned long long e = s.list[i];
                 const uint32_t v = ~(uint32_t)(t.rank ? e : e >> 32), p = v - shift;
                 if (p < span.lo || p >= span.hi || v < sl.lo || v - sl.lo >= sl.len) continue;
-                if (t.rank == 0) mass += (double)__uint_as_float((uint32_t)e);
+                if (t.rank == 0) mass += (double)__uint_as_float((uint32_t)e) * unit;
                 else if (const float x = value_of((uint32_t)(e >> 32)); kept.has(x, v)) mass += (double)w.quick(x) * unit;
             }
             mass = warp_sum(mass);
