@@ -1187,8 +1187,10 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
         }
         if (t.warp < (quick_k ? 4 : quick_p ? 2 : 0)) {
             // cut[l]: at least top_k / 2^l of this slice are not below it.  The largest keys by their upper half that so many threads' largest x have.
-            // For top_p: as many as are this CTA's part of 64 and of 256, and in cut[2 + l] what they weigh (not less).
-            const uint32_t wanted = quick_k ? (set.top_k + (1u << t.warp) - 1u) >> t.warp : ((t.warp ? SM_QUICK_P1 : SM_QUICK_P0) + t.C - 1u) / t.C;
+            // For top_p: as many as are this CTA's part of 64 and of 256, and in cut[2 + l] what they weigh (not less); of a slice with fewer tokens
+            // that are allowed, all.
+            const uint32_t of_row = t.warp ? SM_QUICK_P1 : SM_QUICK_P0;
+            const uint32_t wanted = quick_k ? (set.top_k + (1u << t.warp) - 1u) >> t.warp : min((of_row + t.C - 1u) / t.C, (of_row * sl.len + vocab - 1u) / vocab);
             uint32_t k[SM_THREADS / 32], most = 0u, least = 0xFFFFu;
 #pragma unroll
             for (int i = 0; i < SM_THREADS / 32; i++) {
@@ -1210,11 +1212,21 @@ k_sample(const __grid_constant__ b200bpe_logits in, const __grid_constant__ b200
             if (most == least && wanted <= SM_THREADS) cut = most;
             if (t.lane == 0 && cut > LOWEST_KEY >> 16) s.cut[t.warp] = value_of(cut << 16);
             if (quick_p) {
+                // (the upper half of -infinity's key, of a thread without an allowed token, is a NaN's)
                 double weight = 0;
+                uint32_t lowest = 0xFF80u;           // of infinity, where no token is allowed
 #pragma unroll
-                for (int i = 0; i < SM_THREADS / 32; i++) weight += k[i] >= cut ? (double)Stats::two_to(fmaf(value_of(k[i] << 16), stats.c, -n)) : 0.0;
+                for (int i = 0; i < SM_THREADS / 32; i++)
+                    if (k[i] > LOWEST_KEY >> 16 && k[i] >= cut) {
+                        weight += (double)Stats::two_to(fmaf(value_of(k[i] << 16), stats.c, -n));
+                        lowest = min(lowest, k[i]);
+                    }
                 weight = warp_sum(weight);
-                if (t.lane == 0) s.cut[2 + t.warp] = (float)weight;
+                lowest = __reduce_min_sync(0xFFFFFFFFu, lowest);
+                if (t.lane == 0) {
+                    s.cut[t.warp] = value_of(lowest << 16);
+                    s.cut[2 + t.warp] = (float)weight;
+                }
             }
         }
         __syncthreads();
