@@ -161,7 +161,7 @@ k_grammar_advance(const __grid_constant__ GrammarTables g, const uint32_t* state
     }
     if (t != B200BPE_NO_TOKEN) {
         uint32_t to = GR_DEAD;
-        if (state < g.states && t == g.end_token) to = g.accepting[state] ? state : GR_DEAD;
+        if (state < g.states && t < g.entries && t == g.end_token) to = g.accepting[state] ? state : GR_DEAD;
         else if (state < g.states && t < g.entries && g.entry[t].len) to = walk(g, state, g.entry[t], 0);
         state = to == GR_DEAD ? B200BPE_NO_STATE : to;
     }
