@@ -10,7 +10,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from .token_sampler import IDS, raw_stream, row_of, table_of
+from .token_sampler import IDS, _refuse, raw_stream, row_of, table_of
 
 
 class TokenGrammar:
@@ -50,7 +50,9 @@ class TokenGrammar:
         """states [rows] → mask int32 [rows, (vocabSize + 31) // 32] (or `out`, at least as wide): the tokens with bytes, all of which the automaton
         takes from the row's state, and the end token in an accepting state.  A state that is none (-1) allows nothing."""
         stream, at = self._ready(), self._engine.device_index
-        shape, words = states.shape[:1], (self.vocabSize + 31) >> 5
+        shape, words = getattr(states, "shape", ())[:1], (self.vocabSize + 31) >> 5
+        if not shape:
+            _refuse(states, "states", at, IDS, (None,))
         address = row_of(states, "states", at, IDS, shape)
         rows = shape[0]
         if out is None:
@@ -75,8 +77,10 @@ class TokenGrammar:
         With history [rows, room] and lengths: tokens are also written behind each row's history, and → (states, new lengths) (or
         `lengthsOut`, which may be lengths).  No token, and a full row, changes neither."""
         stream, at = self._ready(), self._engine.device_index
-        shape = states.shape[:1]
-        rows = shape[0] if shape else 0
+        shape = getattr(states, "shape", ())[:1]
+        if not shape:
+            _refuse(states, "states", at, IDS, (None,))
+        rows = shape[0]
         p_states, p_tokens = row_of(states, "states", at, IDS, shape), row_of(tokens, "tokens", at, IDS, shape)
         if out is None:
             import torch
