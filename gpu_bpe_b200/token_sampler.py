@@ -86,6 +86,8 @@ class TokenSampler:
         index = self._engine.device_index
         if isinstance(value, (int, float)):
             import torch
+            if kinds is IDS and not (-2**31 <= value < 2**31 and value == int(value)):
+                raise ValueError(f"{name}: a whole number of 32 bits is needed")
             value = torch.full(shape, value, dtype=torch.int32 if kinds is IDS else torch.float32, device=f"cuda:{index}")
             keep.append(value)
         return row_of(value, name, index, kinds, shape)
