@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t walk(const GrammarTables& g, uint32_t state,
 }
 
 // A CTA makes the words of GR_TILE tokens for some rows.  256 rows of 64,256 entries, an automaton of 205 states and 36 classes: 26 us, where a walk for
-// each token and row took 74; 1,500 rows of 32,256 entries: 54 us, against 200.  Of those 256 rows' pairs 93 % die at their first byte, 3 % stay where they are,
+// each token and row took 74; 1,500 rows of 32,256 entries: 57 us, against 200.  Of those 256 rows' pairs 93 % die at their first byte, 3 % stay where they are,
 // and 4 % are looked at further.  The memory's part is below a microsecond; what bounds it is instructions (14.5 million of warps, 13 us if none waited)
 // and the scattered look-ups of the walks.
 __global__ void __launch_bounds__(GR_THREADS, 8)
@@ -317,7 +317,9 @@ b200bpe_status b200bpe_grammar_mask(b200bpe_grammar* h, const uint32_t* states, 
     const OnDevice on(h->g.ctx->device);
     B2_CUDA(on.error);
     // Rows of a CTA: some states have many times the work of others, so that few rows each share the work out better, and many load the entries less
-    // often.  63 tiles, 256 rows: 24.7 us with 4, 31.3 with 8, 34.4 with 16; 32 tiles, 1,500 rows: 61.2, 58.5, 56.2.
+    // often, which pays once there are CTAs for every place on the GPU (148 SMs with eight) about twice over.  63 tiles and 256 rows: 30.6 us with 4, 38.9 with 8,
+    // 38.4 with 16; 512 rows: 45.6, 43.5, 48.1; 1,024: 86.7, 72.1, 65.4.  32 tiles and 512 rows: 26.5, 31.4, 34.1; 1,024: 47.2, 39.8, 38.8.  (Fewer than 4 gain a
+    // quarter with few tiles and cost it with many: 4 tiles and 256 rows 7.6 us with 2 and 9.8 with 4, 63 tiles 34.9 and 30.6.)
     const uint32_t tiles = (g.entries + GR_TILE - 1) / GR_TILE;
     uint32_t each = GR_ROWS;
     while (each > 4 && (uint64_t)tiles * ((n_rows + each - 1) / each) < 2560) each /= 2;

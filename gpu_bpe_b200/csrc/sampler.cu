@@ -125,7 +125,9 @@ struct Special {
 // Makes `special`, and x of the places in the history and of those with a bias: so these cost a scattered load a token, not a test and a division for
 // every lane of the row.  Returns whether there are any special places.  Called by all threads of the CTA; ends with a barrier.
 // Each CTA reads the whole history of its row, and counts what is its own: a history is short beside a row, and L2 has it.  What a thread reads first
-// does not depend on anything else that is read, so that a row's settings and the first of its history are one wait.
+// does not depend on anything else that is read, so that a row's settings and the first of its history are one wait.  Up to 2,048 tokens stay in
+// registers; a longer history is passed over three times.  256 rows of 131,072 in 16 bits, adjusted: 27 us without a history, 46 with one of 1,500 tokens, 50
+// with 2,048, 70 with 2,049, 122 with 4,000 and 854 with 32,768: where histories are as long as prompts, they are what bounds the call.
 template <uint32_t MOST, class T>
 __device__ __forceinline__ bool find_special(const b200bpe_logits& in, uint32_t vocab, const T* row, const Slice& s, const MaskRow& mask, Special<MOST>& special) {
     constexpr int EACH = 8;                          // of a history, a thread keeps at hand
@@ -317,8 +319,8 @@ __device__ __forceinline__ void write_out(T* to, const Slice& s, bool alike, uin
 }
 
 // A CTA for each slice of a row.  Bound by memory: a row is read and written once, and its special places are few.  256 rows of 131,072 in 32 bits
-// (268 MB: 41 us at the memory's rate): 42 us; with masks and biases 50; with histories of 1,500 tokens 60, all together 66, of which what is above 42 is the
-// wait for a history, its count and the scattered logits of its tokens, while a quarter of a CTA's loads are on their way.
+// (268 MB: 41 us at the memory's rate): 42 us; with masks and biases 50; with histories of 1,500 tokens 60, all together 65, of which what is above 42 is the
+// wait for a history, its count and the scattered logits of its tokens, while half of a CTA's loads are on their way (4,096 of 8,192 values in 32 bits).
 template <class T>
 __global__ void __launch_bounds__(SM_THREADS, 4)
 k_adjust(const __grid_constant__ b200bpe_logits in, uint32_t vocab, uint32_t whole, T* out, uint64_t out_stride) {
@@ -339,7 +341,9 @@ k_adjust(const __grid_constant__ b200bpe_logits in, uint32_t vocab, uint32_t who
 
 // ── the choice ──
 // A thread's largest x, the place of the first vector that has it, and the sum of 2^(x c - n) over its x, n being a whole number next to the largest
-// x c: sums with different n are brought to one another by powers of two, without rounding.
+// x c: sums with different n are brought to one another by powers of two, without rounding.  Weights have 32 bits here, since 64 for every x of the row would
+// be bound by arithmetic (the first version: 398 us for 128 rows of 262,144, 117 now).  A logprob is made of their sum: it is off by at most 2^-22 + 3 * 2^-24 ln(vocabulary)
+// before it is rounded to 32 bits.  What they decide is looked at again where it is near (below).
 struct Stats {
     // 2^25: up to there the whole number is within 1 of x c (half of a step between floats; further out a weight of the largest x itself could be 2^256).
     static constexpr float FAR = 33554432.0f;
@@ -853,7 +857,7 @@ struct Settings {
 };
 
 // The part of the row's order at which a running sum, from the largest x on, reaches `target`: of weights (MASS) or of tokens.
-// s.bins are filled in all CTAs (weights: in parts of 2^16 of the bin's largest), and a barrier of the cluster is behind that.
+// s.bins are filled in all CTAs (weights: in parts of 2^16 of that of the bin's middle), and a barrier of the cluster is behind that.
 // Returns what is kept up to and with the token that reaches it, the same in every CTA.  With `set` (nothing was taken away before) `found` is where the
 // draw falls, if that is known by the way; the caller has its owner at 0xFFFFFFFF.
 template <bool MASS>

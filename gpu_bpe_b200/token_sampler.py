@@ -149,7 +149,8 @@ class TokenSampler:
         (may be logits; of the same type; columns behind the vocabulary are left as they are) or a new tensor [rows, vocabSize].
 
         history [rows, room] holds each row's tokens so far, lengths says how many, promptLengths how many of them were given (they count for
-        repetition, not for presence and frequency).  repetition, presence, frequency: one number a row, or one for all.
+        repetition, not for presence and frequency).  repetition, presence, frequency: one number a row, or one for all (which makes a tensor, a kernel
+        of its own, in every call: a loop keeps tensors).
         biasTokens, biases [rows, n]: ids (-1: unused place) and what is added.  mask [rows, words]: bit v & 31 of word v >> 5 allows token v, as
         TokenGrammar.allowedTokens makes them; with maskRows, row maskRows[r] of it is row r's, and none allows anything."""
         keep = []
@@ -175,7 +176,7 @@ class TokenSampler:
         Without uniform every row takes its largest adjusted logit.  With uniform [rows] in [0, 1): of the topK largest (0: all), of those the shortest
         run from the largest on that has topP of their weight exp(x / temperature), of those the ones with at least minP times the largest weight,
         the first in order of ids at which the running sum of weights is above uniform times their sum.  temperature below
-        2^-16: the largest.  Each is one number a row, or one for all.  logprobs are under the weights of all allowed tokens (at temperature 1
+        2^-16: the largest.  Each but uniform is one number a row, or one for all, as in adjustLogits.  logprobs are under the weights of all allowed tokens (at temperature 1
         where the largest is taken).  A row without an allowed token gives -1 and -inf; a NaN is never chosen."""
         keep = []
         rows, p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
