@@ -154,7 +154,7 @@ class TrieTokenizer:
         out = bytearray()
         for t in tokens:
             t = int(t)
-            out += bytes(self._vocab[t] if 0 <= t < len(self._vocab) else UTF8_REPLACEMENT)
+            out += bytes(self._vocab[t] if t < len(self._vocab) else UTF8_REPLACEMENT)
         return bytes(out)
 
     def sampler(self):
