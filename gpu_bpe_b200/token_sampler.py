@@ -177,7 +177,8 @@ class TokenSampler:
         run from the largest on that has topP of their weight exp(x / temperature), of those the ones with at least minP times the largest weight,
         the first in order of ids at which the running sum of weights is above uniform times their sum.  temperature below
         2^-16: the largest.  Each but uniform is one number a row, or one for all, as in adjustLogits.  logprobs are under the weights of all allowed tokens (at temperature 1
-        where the largest is taken).  A row without an allowed token gives -1 and -inf; a NaN is never chosen."""
+        where the largest is taken).  A row without an allowed token gives -1 and -inf (TrieTokenizer.decode counts
+        negative ids from the vocabulary's end: it is not given a -1); a NaN is never chosen."""
         keep = []
         rows, p = self._logits(keep, logits, history, lengths, promptLengths, repetition, presence, frequency, biasTokens, biases, mask, maskRows)
         shape = logits.shape[:1]
